@@ -510,6 +510,50 @@ int apus_cuda_sparse_attn_batch_dev(const float *q, const float *sink, int h, in
                                     const uint16_t *kv_b, int64_t nb, int64_t kv_b_stride,
                                     float *o, void *stream);
 
+/* ---- latent caches held in 8 bits (no counterpart in the reference, which keeps f32 rows) ------
+ * A cache row is one latent vector of d channels, key and value at once, shared by all heads
+ * (c/attn.h:147-160).  It is held as a record of apus_cuda_kv8_row_bytes(d, rd) = d + rd + 16
+ * bytes -- 592 at d = 512, rd = 64, against 2,048 as f32 and 1,024 as BF16:
+ *   [d - rd E4M3 codes][rd BF16: the rotated channels][one UE8M0 scale per 64 codes, zeros]
+ * Codes and scales are those of apus_cuda_fp8_qat_sim (c/attn.h:290-369), so rows that have been
+ * through it, as the model's window rows and compressed entries have, are held exactly.  A group
+ * of 64 with an infinity or a NaN in it reads back as NaN.  d: a multiple of 64 up to 512; rd: 0
+ * or 64, below d (0 bytes and a message otherwise).
+ * A cache is the caller's device memory: n_seq sequences of `cap` records, sequence b from record
+ * b * stride on.  All pointers are device pointers and start on 16-byte boundaries (pos, counts,
+ * idx, idxs and sink on their types'); work is enqueued on `stream`, nothing is kept between
+ * calls and no memory is allocated, so calls may run side by side and be recorded into graphs. */
+size_t apus_cuda_kv8_row_bytes(int d, int rd);
+/* Quantises x [n_seq, s, d] (f32, or BF16 when x_bf16) into the caches: row t of sequence b goes to
+ * entry pos[b] + t (pos [n_seq], on the device), modulo cap when `ring`.  counts [n_seq]
+ * (nullable): only the first counts[b] rows of sequence b are real, the padding behind them is
+ * left alone.  Rows that no entry takes (a negative one; at cap or behind it without `ring`) are
+ * dropped; of rows that share a place in a ring the last one stays, as if they were written one
+ * by one.  Entries that no row goes to keep their bytes.  n_seq > 1 needs stride >= cap. */
+int apus_cuda_kv8_write_dev(const void *x, int x_bf16, int d, int rd, int n_seq, int s,
+                            const int64_t *pos, const int32_t *counts, int ring,
+                            uint8_t *cache, int64_t cap, int64_t stride, void *stream);
+/* out [n_seq, s, d] (f32, or BF16 when out_bf16; the same values) = the rows that entries
+ * idx[b, t] of sequence b stand for (idx [n_seq, s]), or entries first + t when idx is NULL; an
+ * entry outside 0 .. cap - 1 gives a row of zeros.  stride 0: one cache for all sequences. */
+int apus_cuda_kv8_read_dev(const uint8_t *cache, int d, int rd, int64_t cap, int64_t stride,
+                           int n_seq, int s, const int32_t *idx, int64_t first, void *out,
+                           int out_bf16, void *stream);
+/* apus_cuda_sparse_attn_batch_dev over such caches: q [rows, h, d] (f32 that is rounded to BF16, or
+ * BF16 when q_bf16), idxs [rows, idxw], query row r belongs to sequence r / rows_per_seq (1: a
+ * decode step; the chunk length: a prompt, [n_seq, rows_per_seq] rows).  An id below na is a record
+ * of kv_a, from na on one of kv_b; a negative id, or one at na + nb or behind it, is a hole.  sink
+ * [h] may be NULL: no sink.  o [rows, h, d]: BF16 values, as f32 or (o_bf16) BF16; zeros for a row
+ * of holes.  Strides in records (0: one cache for all sequences).  The contractions run on the tensor
+ * cores (BF16 products, f32 sums in their order) and the softmax numerators are BF16 as in
+ * c/attn.h:1308, so a result is within a BF16 step or two of the reference's, not its bits.  The
+ * same call gives the same bits. */
+int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const float *sink, int h, int d,
+                                  int rd, const int32_t *idxs, int idxw, int rows,
+                                  int rows_per_seq, float scale, const uint8_t *kv_a, int64_t na,
+                                  int64_t kv_a_stride, const uint8_t *kv_b, int64_t nb,
+                                  int64_t kv_b_stride, void *o, int o_bf16, void *stream);
+
 /* ---- block and model (c/layer.h, c/model.h) --------------------------------- */
 
 /* The fields of the reference's ApusLayer (c/layer.h:45-71) that
