@@ -29,13 +29,35 @@ struct AttnKv8Args {
     int *status;
 };
 
-// The record that id `id` of sequence `seq` names, NULL for a hole.
-__device__ __forceinline__ const uint8_t *kv8_record(const AttnKv8Args &a, long long seq, int id) {
-    if (id < 0) return nullptr;
-    const size_t rb = (size_t)kv8_row_bytes(a.d, a.rd);
-    if (id < a.na) return a.kv_a + (size_t)(seq * a.a_stride + id) * rb;
-    const long long j = id - a.na;
-    return j < a.nb ? a.kv_b + (size_t)(seq * a.b_stride + j) * rb : nullptr;
+// Where a sequence's records lie: id i below na at a + i * bytes, others at b + i * bytes.
+struct Kv8Seq {
+    uintptr_t a, b;
+    int na, n;                                          // ids from n on are holes
+    uint32_t bytes;
+    __device__ __forceinline__ Kv8Seq(const AttnKv8Args &p, long long seq) {
+        bytes = (uint32_t)kv8_row_bytes(p.d, p.rd);
+        a = (uintptr_t)p.kv_a + (uintptr_t)(seq * p.a_stride) * bytes;
+        b = (uintptr_t)p.kv_b + (uintptr_t)(seq * p.b_stride - p.na) * bytes;
+        na = (int)p.na;
+        n = (int)(p.na + p.nb);
+    }
+    __device__ __forceinline__ const uint8_t *at(int id) const {      // id not a hole
+        return reinterpret_cast<const uint8_t *>((id < na ? a : b) + (uintptr_t)(uint32_t)id * bytes);
+    }
+};
+// 16 or 8 bytes of global memory, or zeros; here and not where the value is first used, and without a branch
+__device__ __forceinline__ uint4 ldg16_if(const uint8_t *p, bool yes) {
+    uint4 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+                 "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((uint32_t)yes));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8_if(const uint8_t *p, bool yes) {
+    uint2 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"((uint32_t)yes));
+    return v;
 }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
@@ -59,27 +81,33 @@ __device__ __forceinline__ const uint8_t *kv8_record(const AttnKv8Args &a, long 
 // tells the others its references and sums, scales its part of O^T and stores it into the shared memory of the CTA that
 // owns the channels, which adds the parts in rank order: one launch, no scratch, the same bits every time.
 //
-// Warps 0 to 7 fetch (into registers, a tile ahead), dequantise and do the softmax; warp 8 issues the MMAs.  Shared
-// memory: 8 panels of 128 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64 heads x 64 channels, P.
-constexpr int AK_TILE = 128, AK_HEADS = 64, AK_WORKERS = 256, AK_THREADS = AK_WORKERS + 32, AK_MAX_C = 16;
+// Warps 0 to 3: queries, softmax.  Warps 4 to 11: rows, fetched into registers a tile ahead and dequantised into shared
+// memory; the output at the end.  Warp 12 issues the MMAs.  Thirteen warps have 128 registers a thread, which is what both
+// the softmax (64 sums) and the rows (72 registers in flight) need; with fewer, larger roles they spilt, and what is spilt here
+// goes to L2, since shared memory leaves no L1.  Shared memory: 8 panels of 128 tokens x 64 channels (128-byte swizzled
+// rows), Q as 8 panels of 64 heads x 64 channels, P.
+constexpr int AK_TILE = 128, AK_HEADS = 64, AK_MAX_C = 16;
+constexpr int AK_SOFT = 4, AK_ROWS = 8, AK_MMA = AK_SOFT + AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + AK_PANEL;
-constexpr float AK_SLACK = 40.f, AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
+constexpr uint32_t AK_SLACK = 40;
+constexpr float AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 
 struct AkMisc {
     float2 ml[AK_MAX_C][AK_HEADS];                     // reference and sum of every CTA of the cluster
     float m[AK_HEADS], f[AK_HEADS], part[4][AK_HEADS];
-    uint64_t full[4], empty[4], s_full, p_ready, o_done;
+    uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
 };
 constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc) + 1024;
 static_assert(AK_SMEM <= 227 * 1024, "shared memory of a CTA");
 
-__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ bool workers_any(bool p) {
+// barriers of the softmax warps
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool soft_any(bool p) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(r) : "r"((uint32_t)p) : "memory");
     return r != 0;
 }
@@ -89,6 +117,10 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+// A wait of a whole warp, which goes on together
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -104,6 +136,11 @@ __device__ __forceinline__ float redux_max(float x) {
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -122,12 +159,21 @@ __device__ __forceinline__ uint32_t ak_idesc(bool mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (mn ? (1u << 15) | (1u << 16) : 0u) | ((uint32_t)(AK_HEADS >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
 }
+// Issued by one lane of a whole, converged warp: with no branch around it the descriptors stay in uniform registers.
 __device__ __forceinline__ void ak_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void ak_commit(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_u32(bar)) : "memory");
 }
 // MN-major operand of 128-byte swizzled rows, a row per k: 64 elements of M or N in a row, the next 64 a panel further
 __device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr) {
@@ -135,28 +181,31 @@ __device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr) {
            (uint64_t)2 << 61;
 }
 
-// Four codes -> four BF16 values times 2^-120: sign, exponent and significand bits moved to their places (the biases of
-// the two formats differ by 120; a subnormal code becomes a subnormal value).
-__device__ __forceinline__ uint2 codes_bf16x4(uint32_t c) {
-    const uint32_t a = __byte_perm(c, 0u, 0x1404), b = __byte_perm(c, 0u, 0x3424);
-    return make_uint2((a & 0x80008000u) | (a >> 4 & 0x07f007f0u), (b & 0x80008000u) | (b >> 4 & 0x07f007f0u));
+// Four codes -> four BF16 values in the order 0 2 | 1 3, times 2^120 the factor in `f` (a BF16 value twice).  Exponent and
+// significand move to their places in BF16 (whose bias is 120 larger; a subnormal code becomes a subnormal value) and the
+// sign goes into the factor.  The order saves the byte permutations: integer instructions issue every other cycle, and they
+// bound this (64 codes of a lane: 330 -> 200 cycles of a scheduler).  Queries and output channels follow it (ak_order).
+__device__ __forceinline__ uint2 codes_bf16x4(uint32_t c, uint32_t f) {
+    return make_uint2(mul_bf16x2(c << 4 & 0x07f007f0u, (c << 8 & 0x80008000u) | f), mul_bf16x2(c >> 4 & 0x07f007f0u, (c & 0x80008000u) | f));
 }
+__device__ __forceinline__ int ak_order(int ch) { return (ch & ~3) | (ch & 1) << 1 | (ch >> 1 & 1); }
 // 16 codes of a group with scale byte `b` -> 16 BF16 values.  2^120 times the scale is a BF16 value up to byte 134 (rows of
 // magnitude 57,344); larger ones take two multiplications.
 __device__ __forceinline__ void dequant16(const uint4 &c, uint32_t b, uint4 &lo, uint4 &hi) {
-    const uint2 w0 = codes_bf16x4(c.x), w1 = codes_bf16x4(c.y), w2 = codes_bf16x4(c.z), w3 = codes_bf16x4(c.w);
+    const uint32_t f = b <= 134u ? b * 0x00800080u + 0x3c003c00u : 0x7b807b80u;
+    const uint2 w0 = codes_bf16x4(c.x, f), w1 = codes_bf16x4(c.y, f), w2 = codes_bf16x4(c.z, f), w3 = codes_bf16x4(c.w, f);
     lo = make_uint4(w0.x, w0.y, w1.x, w1.y);
     hi = make_uint4(w2.x, w2.y, w3.x, w3.y);
-    uint32_t f = (b + 120u) << 7;
     if (b > 134u) {
-        const uint32_t up = (247u << 7) | (247u << 23);
-        lo = make_uint4(mul_bf16x2(lo.x, up), mul_bf16x2(lo.y, up), mul_bf16x2(lo.z, up), mul_bf16x2(lo.w, up));
-        hi = make_uint4(mul_bf16x2(hi.x, up), mul_bf16x2(hi.y, up), mul_bf16x2(hi.z, up), mul_bf16x2(hi.w, up));
-        f = b == 255u ? 0x7fffu : b << 7;
+        const uint32_t g = b == 255u ? 0x7fff7fffu : b * 0x00800080u;
+        lo = make_uint4(mul_bf16x2(lo.x, g), mul_bf16x2(lo.y, g), mul_bf16x2(lo.z, g), mul_bf16x2(lo.w, g));
+        hi = make_uint4(mul_bf16x2(hi.x, g), mul_bf16x2(hi.y, g), mul_bf16x2(hi.z, g), mul_bf16x2(hi.w, g));
     }
-    f |= f << 16;
-    lo = make_uint4(mul_bf16x2(lo.x, f), mul_bf16x2(lo.y, f), mul_bf16x2(lo.z, f), mul_bf16x2(lo.w, f));
-    hi = make_uint4(mul_bf16x2(hi.x, f), mul_bf16x2(hi.y, f), mul_bf16x2(hi.z, f), mul_bf16x2(hi.w, f));
+}
+// 16 bytes to shared memory.  No memory clobber: the loads that follow in the program need not wait for it (every use of what
+// is stored lies behind a fence or a barrier that has one).
+__device__ __forceinline__ void sts16(void *p, const uint4 &v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(p)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
 }
 
 // The ids of a tile, token 32 k + lane in id[k]; whether any of them names a record is the same in every warp.
@@ -167,69 +216,70 @@ struct TileIds {
 #pragma unroll
         for (int k = 0; k < 4; k++) id[k] = t0 + 32 * k + lane < t1 ? ids[t0 + 32 * k + lane] : -1;
     }
-    __device__ __forceinline__ bool any(const AttnKv8Args &a) {
-        bool v = false;
+    __device__ __forceinline__ bool any(int n) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (id[k] >= a.na + a.nb) id[k] = -1;
-            v |= id[k] >= 0;
-        }
-        return __any_sync(0xffffffffu, v);
+        for (int k = 0; k < 4; k++) id[k] = id[k] < n ? id[k] : -1;
+        return __any_sync(0xffffffffu, max(max(id[0], id[1]), max(id[2], id[3])) >= 0);
     }
 };
 
-// What a worker lane fetches of a tile: of its rows r0 and r0 + 8, 16 channels of every panel of codes, 16 BF16 values of
-// the rotated panel and the scales.
+// What a lane of the row warps holds of a tile: of its rows r0 and r0 + 8, 16 channels of every panel of codes (or 16 BF16
+// values of the rotated panel, in the place of two), and the scales.
 template <bool TAIL>
 struct TileRows {
     static constexpr int NC = TAIL ? 7 : 8;
-    const uint8_t *rec[2];
-    uint4 c[NC][2], t[TAIL ? 2 : 1][2];
+    uint4 c[NC][2], t[2][TAIL ? 2 : 1];
     uint2 sc[2];
-    __device__ __forceinline__ void find(const AttnKv8Args &a, long long seq, const TileIds &ids, int warp, int lane) {
-        const int src = (warp & 1) * 16 + (lane >> 2);
-        const int mine = warp >> 1 == 0 ? ids.id[0] : warp >> 1 == 1 ? ids.id[1] : warp >> 1 == 2 ? ids.id[2] : ids.id[3];
-#pragma unroll
-        for (int i = 0; i < 2; i++) rec[i] = kv8_record(a, seq, __shfl_sync(0xffffffffu, mine, src + 8 * i));
-    }
-    // panels 0 to 3 and the scales, or the others
-    template <bool FIRST>
-    __device__ __forceinline__ void load(const AttnKv8Args &a, int sub) {
-        const int nq = a.d - a.rd;
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const uint8_t *rec[2];                              // of the tile that is fetched
+    bool is[2];
+    __device__ __forceinline__ void find(const Kv8Seq &at, const TileIds &ids, int w, int lane) {
+        const int src = (w & 1) * 16 + (lane >> 2);
+        const int mine = w >> 1 == 0 ? ids.id[0] : w >> 1 == 1 ? ids.id[1] : w >> 1 == 2 ? ids.id[2] : ids.id[3];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint8_t *r = rec[i];
-#pragma unroll
-            for (int p = FIRST ? 0 : 4; p < (FIRST ? 4 : NC); p++) c[p][i] = r && p * 64 < nq ? *reinterpret_cast<const uint4 *>(r + p * 64 + sub * 16) : zero;
-            if (TAIL && !FIRST) {
-                t[0][i] = r ? *reinterpret_cast<const uint4 *>(r + nq + sub * 32) : zero;
-                t[TAIL ? 1 : 0][i] = r ? *reinterpret_cast<const uint4 *>(r + nq + sub * 32 + 16) : zero;
-            }
-            if (FIRST) sc[i] = r ? *reinterpret_cast<const uint2 *>(r + kv8_scale_off(a.d, a.rd)) : make_uint2(0u, 0u);
+            const int id = __shfl_sync(0xffffffffu, mine, src + 8 * i);
+            is[i] = id >= 0;
+            rec[i] = at.at(id);
         }
     }
-    // panel p of the tile into shared memory, rows r0 and r0 + 8
+    __device__ __forceinline__ void load_scales(int off) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) sc[i] = ldg8_if(rec[i] + off, is[i]);
+    }
+    // `nq`: channels held as codes
+    __device__ __forceinline__ void load(int nq, int p, bool rotated, int sub) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (TAIL && rotated) {
+                t[i][0] = ldg16_if(rec[i] + nq + sub * 32, is[i]);
+                t[i][TAIL ? 1 : 0] = ldg16_if(rec[i] + nq + sub * 32 + 16, is[i]);
+            } else {
+                c[p < NC ? p : 0][i] = ldg16_if(rec[i] + p * 64 + sub * 16, is[i]);
+            }
+        }
+    }
+    // panel p of the tile into shared memory
     __device__ __forceinline__ void store(uint8_t *panel, int p, bool rotated, int r0, int sub) const {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             uint4 lo, hi;
             if (TAIL && rotated) {
-                lo = t[0][i];
-                hi = t[TAIL ? 1 : 0][i];
+                lo = t[i][0];
+                hi = t[i][TAIL ? 1 : 0];
             } else {
                 dequant16(c[p < NC ? p : 0][i], (p < 4 ? sc[i].x >> 8 * (p & 3) : sc[i].y >> 8 * (p & 3)) & 0xffu, lo, hi);
             }
             uint8_t *row = panel + (r0 + 8 * i) * 128;
-            *reinterpret_cast<uint4 *>(row + ((2 * sub) ^ (r0 & 7)) * 16) = lo;
-            *reinterpret_cast<uint4 *>(row + ((2 * sub + 1) ^ (r0 & 7)) * 16) = hi;
+            sts16(row + ((2 * sub) ^ (r0 & 7)) * 16, lo);
+            sts16(row + ((2 * sub + 1) ^ (r0 & 7)) * 16, hi);
         }
     }
 };
 
-// o[head][ch] of one warp: lane = channel, v[i] = head h0 + i of it, already scaled
+// o[head][ch] of one warp: lane = channel ch, v[i] = head h0 + i of it, already scaled; `mate`: the lane with the other channel
+// of an even and odd pair is lane ^ mate
 template <int N>
-__device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, int h0, int nh, const float (&v)[N], int lane) {
+__device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, int mate, int h0, int nh, const float (&v)[N]) {
     if (!a.o_bf16) {
         float *o = static_cast<float *>(a.o) + at + ch + (size_t)h0 * a.d;
 #pragma unroll
@@ -237,13 +287,14 @@ __device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, 
             if (h0 + i < nh) *o = __uint_as_float(bf16x2_rn(v[i], 0.f) << 16);
         return;
     }
-    // two lanes trade, so that each stores two channels of one of two heads
-    uint16_t *o = static_cast<uint16_t *>(a.o) + at + (ch & ~1) + (size_t)(h0 + (lane & 1)) * a.d;
+    // the two lanes trade, so that each stores both channels of one of two heads
+    const bool odd = ch & 1;
+    uint16_t *o = static_cast<uint16_t *>(a.o) + at + (ch & ~1) + (size_t)(h0 + odd) * a.d;
 #pragma unroll
     for (int i = 0; i < N; i += 2, o += 2 * a.d) {
-        const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 1], 1);
-        const uint32_t w = lane & 1 ? bf16x2_rn(other, v[i + 1]) : bf16x2_rn(v[i], other);
-        if (h0 + i + (lane & 1) < nh) *reinterpret_cast<uint32_t *>(o) = w;
+        const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], mate);
+        const uint32_t w = odd ? bf16x2_rn(other, v[i + 1]) : bf16x2_rn(v[i], other);
+        if (h0 + i + odd < nh) *reinterpret_cast<uint32_t *>(o) = w;
     }
 }
 
@@ -259,19 +310,21 @@ attn_kv8_kernel(const AttnKv8Args a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = a.cluster;
     const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * AK_HEADS, nh = min(AK_HEADS, a.h - h0);
     const long long row = blockIdx.x / (unsigned)C, seq = row / a.rows_per_seq;
+    const Kv8Seq at(a, seq);
     const int32_t *ids = a.idxs + (size_t)row * a.idxw;
     const int n_tiles = (a.idxw + a.unit - 1) / a.unit, NP = a.d / 64, NPAIR = (NP + 1) / 2;
 
     if (tid == 0) {
-        for (int i = 0; i < 4; i++) { mbar_init(&sm.full[i], 8); mbar_init(&sm.empty[i], 1); }
+        for (int i = 0; i < 4; i++) { mbar_init(&sm.full[i], AK_ROWS); mbar_init(&sm.empty[i], 1); }
+        mbar_init(&sm.q_full, AK_MMA);
         mbar_init(&sm.s_full, 1);
-        mbar_init(&sm.p_ready, 8);
+        mbar_init(&sm.p_ready, AK_SOFT);
         mbar_init(&sm.o_done, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
-    if (warp == 8) {
+    if (warp == AK_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -280,213 +333,250 @@ attn_kv8_kernel(const AttnKv8Args a) {
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (C > 1) cluster_arrive();                        // this CTA has started: its shared memory may be stored to
-    const uint32_t tmem = sm.tmem, tmem_s = tmem + 4 * AK_HEADS;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0), tmem_s = tmem + 4 * AK_HEADS;
 
     // A wait that runs out sets the abort flag, after which every other wait gives up soon; all loops and barriers are gone
     // through all the same, so that no thread is left waiting, and nothing is written.
     int fail = 0;
     uint32_t done = 0;                                   // tiles of this CTA so far
-    TileIds cur;
+    TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
     int tile = rank;
     bool more = false;
-    for (; tile < n_tiles; tile += C) {
-        cur.load(a, ids, tile, lane);
-        if ((more = cur.any(a))) break;
-    }
-
-    if (warp == 8) {
-        const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
-        const uint32_t kv = smem_u32(smem), q = smem_u32(smem + AK_Q_OFF), p = smem_u32(smem + AK_P_OFF);
-        while (more) {
-            const int ks = (min(a.unit, a.idxw - tile * a.unit) + 15) >> 4;      // steps of 16 tokens that hold any
-            if (lane == 0) {
-                for (int i = 0; i < NPAIR && !fail; i++) {
-                    if (!mbar_wait(&sm.full[i], done & 1u, s_abort)) { fail = 51; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    for (int pn = 2 * i; pn < min(2 * i + 2, NP); pn++) {
-                        const uint64_t da = umma_desc_sw128(kv + pn * AK_PANEL), db = umma_desc_sw128(q + pn * AK_QPANEL);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) ak_mma(tmem_s, da + 2 * j, db + 2 * j, id_s, (pn | j) ? 1u : 0u);
-                    }
-                }
-                if (!fail) umma_commit(&sm.s_full);
-                if (!fail && !mbar_wait(&sm.p_ready, done & 1u, s_abort)) fail = 52;
-                if (!fail) {
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    for (int i = 0; i < NPAIR; i++) {
-                        const uint64_t da = ak_desc_mn(kv + 2 * i * AK_PANEL), db = ak_desc_mn(p);
-                        for (int k = 0; k < ks; k++)
-                            ak_mma(tmem + i * AK_HEADS, da + 128 * k, db + 128 * k, id_o, (done | (uint32_t)k) ? 1u : 0u);
-                        umma_commit(&sm.empty[i]);
-                    }
-                }
-                if (fail) *s_abort = 1;
-            }
-            __syncwarp();
-            done++;
-            more = false;
-            for (tile += C; tile < n_tiles; tile += C) {
-                cur.load(a, ids, tile, lane);
-                if ((more = cur.any(a))) break;
-            }
+    auto settle = [&]() {                                // cur has been asked for: the first tile from it on with a record
+        for (more = false; tile < n_tiles; ) {
+            if ((more = cur.any(at.n))) break;
+            tile += C;
+            cur.load(a, ids, tile, lane);
         }
-        if (lane == 0 && !fail) umma_commit(&sm.o_done);
-        __syncwarp();
-    } else {
-        const int r0 = warp * 16 + (lane >> 2), sub = lane & 3, quad = warp & 3, half = warp >> 2, token = quad * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const float cs = a.scale * LOG2E;
-        TileRows<TAIL> rows;
-        rows.rec[0] = rows.rec[1] = nullptr;
-        if (more) rows.find(a, seq, cur, warp, lane);
-        rows.template load<true>(a, sub);
-        // the queries, 8 channels at a time
-        const int per_head = a.d / 8;
-        for (int i0 = 0; i0 < AK_HEADS * per_head; i0 += AK_WORKERS * 4) {
+    };
+    cur.load(a, ids, tile, lane);
+    settle();
+
+    // the queries into shared memory, 8 channels at a time, by all warps but the one of the MMAs
+    auto queries = [&]() {
+        const int per_head = a.d / 8, n = AK_HEADS * per_head, step = 32 * AK_MMA;
+        for (int i0 = tid; i0 < n; i0 += 4 * step) {
             uint4 v[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * AK_WORKERS + tid, head = i / per_head, c = i - head * per_head;
-                v[k] = make_uint4(0u, 0u, 0u, 0u);
-                if (head < nh) {
-                    const size_t at = ((size_t)row * a.h + h0 + head) * a.d + c * 8;
-                    if (a.q_bf16) {
-                        v[k] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at);
-                    } else {
-                        const float4 x = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
-                        const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + 4);
-                        v[k] = make_uint4(bf16x2_rn(x.x, x.y), bf16x2_rn(x.z, x.w), bf16x2_rn(y.x, y.y), bf16x2_rn(y.z, y.w));
-                    }
+                const int i = i0 + k * step, head = i / per_head;
+                const bool there = i < n && head < nh;
+                const size_t from = ((size_t)row * a.h + h0) * a.d + (there ? i : 0) * 8;
+                if (a.q_bf16) {
+                    v[k] = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 2, there);
+                } else {
+                    const uint4 x = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 4, there);
+                    const uint4 y = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 4 + 16, there);
+                    v[k] = make_uint4(bf16x2_rn(__uint_as_float(x.x), __uint_as_float(x.y)), bf16x2_rn(__uint_as_float(x.z), __uint_as_float(x.w)),
+                                      bf16x2_rn(__uint_as_float(y.x), __uint_as_float(y.y)), bf16x2_rn(__uint_as_float(y.z), __uint_as_float(y.w)));
                 }
             }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * AK_WORKERS + tid, head = i / per_head, c = i - head * per_head;
-                if (head < AK_HEADS)
-                    *reinterpret_cast<uint4 *>(smem + AK_Q_OFF + (c >> 3) * AK_QPANEL + head * 128 + (((c & 7) ^ (head & 7)) << 4)) = v[k];
+                const int i = i0 + k * step, head = i / per_head, c = i - head * per_head;
+                if (c * 8 < a.d - a.rd)                  // in the order of the codes
+                    v[k] = make_uint4(__byte_perm(v[k].x, v[k].y, 0x5410), __byte_perm(v[k].x, v[k].y, 0x7632),
+                                      __byte_perm(v[k].z, v[k].w, 0x5410), __byte_perm(v[k].z, v[k].w, 0x7632));
+                if (i < n) sts16(smem + AK_Q_OFF + (c >> 3) * AK_QPANEL + head * 128 + (((c & 7) ^ (head & 7)) << 4), v[k]);
             }
         }
-        float l[32];
+        proxy_fence();
+        mbar_arrive_warp(&sm.q_full, lane);
+    };
+
+    if (warp == AK_MMA) {
+        const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
+        const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
+        const uint64_t dv = ak_desc_mn(smem_u32(smem)), dp = ak_desc_mn(smem_u32(smem + AK_P_OFF));
+        if (!warp_wait(&sm.q_full, 0u, s_abort)) fail = 51;
+        while (more) {
+            const int ks = (min(a.unit, a.idxw - tile * a.unit) + 15) >> 4;      // steps of 16 tokens that hold any
+            tile += C;
+            cur.load(a, ids, tile, lane);
 #pragma unroll
-        for (int i = 0; i < 32; i++) l[i] = 0.f;
+            for (int i = 0; i < 4; i++) {
+                if (i >= NPAIR || fail) break;
+                if (!warp_wait(&sm.full[i], done & 1u, s_abort)) { fail = 52; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int pn = 2 * i; pn < 2 * i + 2; pn++) {
+                    if (pn >= NP) break;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        ak_mma(tmem_s, dk + pn * (AK_PANEL >> 4) + 2 * j, dq + pn * (AK_QPANEL >> 4) + 2 * j, id_s, (pn | j) ? 1u : 0u);
+                }
+            }
+            if (!fail) ak_commit(&sm.s_full);
+            if (!fail && !warp_wait(&sm.p_ready, done & 1u, s_abort)) fail = 53;
+            if (!fail) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (i >= NPAIR) break;
+                    const uint64_t da = dv + 2 * i * (AK_PANEL >> 4);
+                    ak_mma(tmem + i * AK_HEADS, da, dp, id_o, done ? 1u : 0u);
+#pragma unroll
+                    for (int k = 1; k < 8; k++)
+                        if (k < ks) ak_mma(tmem + i * AK_HEADS, da + 128 * k, dp + 128 * k, id_o, 1u);
+                    ak_commit(&sm.empty[i]);
+                }
+            }
+            if (fail) *s_abort = 1;
+            done++;
+            settle();
+        }
+        if (!fail) ak_commit(&sm.o_done);
+    } else if (warp >= AK_SOFT) {
+        const int w = warp - AK_SOFT, r0 = w * 16 + (lane >> 2), sub = lane & 3;
+        TileRows<TAIL> rows;
+        const int nq = a.d - a.rd, scales = kv8_scale_off(a.d, a.rd);
+        auto fetch = [&]() {                             // tile `tile`, all of it
+            rows.find(at, cur, w, lane);
+            rows.load_scales(scales);
+#pragma unroll
+            for (int p = 0; p < 8; p++)
+                if (p < NP) rows.load(nq, p, p == NP - 1, sub);
+        };
+        if (more) fetch();
+        queries();
         while (more) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
-            const int my_id = quad == 0 ? cur.id[0] : quad == 1 ? cur.id[1] : quad == 2 ? cur.id[2] : cur.id[3];
-            const bool valid = my_id >= 0;
-            rows.template load<false>(a, sub);
+            tile += C;
+            cur.load(a, ids, tile, lane);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if (i >= NPAIR) break;
-                if (!mbar_wait(&sm.empty[i], (done & 1u) ^ 1u, s_abort)) fail = 53;
+                if (!warp_wait(&sm.empty[i], (done & 1u) ^ 1u, s_abort)) fail = 54;
                 if (r0 < held) {
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        if (2 * i + k < NP) rows.store(smem + (2 * i + k) * AK_PANEL, 2 * i + k, 2 * i + k == NP - 1, r0, sub);
+                    for (int p = 2 * i; p < 2 * i + 2; p++)
+                        if (p < NP) rows.store(smem + p * AK_PANEL, p, p == NP - 1, r0, sub);
                 }
                 proxy_fence();
                 mbar_arrive_warp(&sm.full[i], lane);
             }
-            // the tile after this one: half of its rows are on their way while the scores are worked on (all of them, and the
-            // scores, are more registers than a thread has)
-            more = false;
-            for (tile += C; tile < n_tiles; tile += C) {
-                cur.load(a, ids, tile, lane);
-                if ((more = cur.any(a))) break;
-            }
-            if (more) {
-                rows.find(a, seq, cur, warp, lane);
-                rows.template load<true>(a, sub);
-            }
-
-            if (!mbar_wait(&sm.s_full, done & 1u, s_abort)) fail = 54;
-            __syncwarp();
+            // The next tile's rows, all at once: they have the softmax and the first MMAs on the values to arrive.  Loads issued
+            // between the stores above would be waited for there, since a thread has few counters of loads in flight.
+            settle();
+            if (more) fetch();
+            if (fail) *s_abort = 1;
+            done++;
+        }
+    } else {
+        const int token = tid;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const float cs = a.scale * LOG2E;
+        queries();
+        // sums of numerators: of 8 heads, over the 8 tokens in a row that this thread adds up of every tile
+        const int lh = tid & 7, lt = (tid >> 3) * 8;
+        float l[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) l[i] = 0.f;
+        uint8_t *prow = smem + AK_P_OFF + token * 128;
+        const float4 *mp = reinterpret_cast<const float4 *>(sm.m);
+        while (more) {
+            const bool valid = (warp == 0 ? cur.id[0] : warp == 1 ? cur.id[1] : warp == 2 ? cur.id[2] : cur.id[3]) >= 0;
+            const uint32_t mask = valid ? ~0u : 0u;      // not a choice: the compiler would branch around every numerator
+            tile += C;
+            cur.load(a, ids, tile, lane);
+            if (!warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[32];
-            tmem_ld32(tmem_s + lanes + half * 32, s);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            const float4 *mp = reinterpret_cast<const float4 *>(sm.m + half * 32);
-            float top = -INFINITY;
+            for (bool set = done == 0;; set = true) {
+                if (set) {
+                    // new references: the maxima over the tokens so far
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float4 m = mp[i];
-                top = fmaxf(top, fmaxf(fmaxf(fmaf(__uint_as_float(s[4 * i]), cs, -m.x), fmaf(__uint_as_float(s[4 * i + 1]), cs, -m.y)),
-                                       fmaxf(fmaf(__uint_as_float(s[4 * i + 2]), cs, -m.z), fmaf(__uint_as_float(s[4 * i + 3]), cs, -m.w))));
-            }
-            if (workers_any(valid && top > AK_SLACK)) {
-                // new references: the maxima over the tokens so far
-                float keep = AK_NONE;
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const float r = redux_max(valid ? __uint_as_float(s[i]) * cs : -INFINITY);
-                    if (lane == i) keep = r;
-                }
-                sm.part[quad][half * 32 + lane] = keep;
-                workers_sync();
-                if (tid < AK_HEADS) {
-                    const float old = sm.m[tid];
-                    const float now = fmaxf(fmaxf(fmaxf(sm.part[0][tid], sm.part[1][tid]), fmaxf(sm.part[2][tid], sm.part[3][tid])), old);
-                    sm.m[tid] = now;
-                    sm.f[tid] = ex2(old - now);
-                }
-                workers_sync();
-                const float *f = sm.f + half * 32;
-#pragma unroll
-                for (int i = 0; i < 32; i++) l[i] *= f[i];
-                if (done) {
-                    for (int i = 0; i < NPAIR; i++) {
-                        uint32_t v[32];
-                        tmem_ld32(tmem + lanes + i * AK_HEADS + half * 32, v);
+                    for (int hf = 0; hf < 2; hf++) {
+                        uint32_t s[32];
+                        tmem_ld32(tmem_s + lanes + 32 * hf, s);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        float keep = AK_NONE;
 #pragma unroll
-                        for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * f[k]);
-                        tmem_st32(tmem + lanes + i * AK_HEADS + half * 32, v);
+                        for (int i = 0; i < 32; i++) {
+                            const float r = redux_max(valid ? __uint_as_float(s[i]) * cs : -INFINITY);
+                            if (lane == i) keep = r;
+                        }
+                        sm.part[warp][32 * hf + lane] = keep;
                     }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                }
-            }
-            uint8_t *prow = smem + AK_P_OFF + token * 128;
+                    soft_sync();
+                    if (tid < AK_HEADS) {
+                        const float old = sm.m[tid];
+                        const float now = fmaxf(fmaxf(fmaxf(sm.part[0][tid], sm.part[1][tid]), fmaxf(sm.part[2][tid], sm.part[3][tid])), old);
+                        sm.m[tid] = now;
+                        sm.f[tid] = ex2(old - now);
+                    }
+                    soft_sync();
+                    if (done) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t w[4];
+                        for (int i = 0; i < 8; i++) l[i] *= sm.f[8 * lh + i];
+                        for (int i = 0; i < 2 * NPAIR; i++) {
+                            uint32_t v[32];
+                            tmem_ld32(tmem + lanes + 32 * i, v);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const float4 m = mp[2 * c + k];
-                    const int i = 8 * c + 4 * k;
-                    const float p0 = valid ? ex2(fmaf(__uint_as_float(s[i]), cs, -m.x)) : 0.f;
-                    const float p1 = valid ? ex2(fmaf(__uint_as_float(s[i + 1]), cs, -m.y)) : 0.f;
-                    const float p2 = valid ? ex2(fmaf(__uint_as_float(s[i + 2]), cs, -m.z)) : 0.f;
-                    const float p3 = valid ? ex2(fmaf(__uint_as_float(s[i + 3]), cs, -m.w)) : 0.f;
-                    w[2 * k] = bf16x2_rn(p0, p1);
-                    w[2 * k + 1] = bf16x2_rn(p2, p3);
-                    // the sum is that of the rounded numerators: the weights then add up to one
-                    l[i] += __uint_as_float(w[2 * k] << 16);
-                    l[i + 1] += __uint_as_float(w[2 * k] & 0xffff0000u);
-                    l[i + 2] += __uint_as_float(w[2 * k + 1] << 16);
-                    l[i + 3] += __uint_as_float(w[2 * k + 1] & 0xffff0000u);
+                            for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * sm.f[32 * (i & 1) + k]);
+                            tmem_st32(tmem + lanes + 32 * i, v);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
                 }
-                *reinterpret_cast<uint4 *>(prow + (((half * 4 + c) ^ (token & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                uint32_t top = 0;                        // the largest numerator: as BF16 bits they compare like numbers
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    uint32_t s[32];
+                    tmem_ld32(tmem_s + lanes + 32 * hf, s);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    // all references before the first store: a load behind a store waits for it to issue, one piece after another
+                    // (64 columns 1,200 cycles; 650 so, of which the exponentials need 512)
+                    float4 m[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) m[i] = mp[8 * hf + i];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const int i = 8 * c + 4 * k;
+                            const float4 r = m[2 * c + k];
+                            w[2 * k] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i]), cs, -r.x)), ex2(fmaf(__uint_as_float(s[i + 1]), cs, -r.y)));
+                            w[2 * k + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[i + 3]), cs, -r.w)));
+                            top = max_u16x2(top, max_u16x2(w[2 * k], w[2 * k + 1]));
+                        }
+                        sts16(prow + (((hf * 4 + c) ^ (token & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                }
+                // a numerator above 2^AK_SLACK: once more with new references
+                if (!soft_any(max(top & 0xffffu, top >> 16) > (127u + AK_SLACK) << 7) || set) break;
             }
             proxy_fence();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive_warp(&sm.p_ready, lane);
+            // while the MMAs run: the sums of the numerators, as they were rounded, so that the weights add up to one
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(smem + AK_P_OFF + (lt + k) * 128 + ((lh ^ k) << 4));
+                l[0] += __uint_as_float(w.x << 16); l[1] += __uint_as_float(w.x & 0xffff0000u);
+                l[2] += __uint_as_float(w.y << 16); l[3] += __uint_as_float(w.y & 0xffff0000u);
+                l[4] += __uint_as_float(w.z << 16); l[5] += __uint_as_float(w.z & 0xffff0000u);
+                l[6] += __uint_as_float(w.w << 16); l[7] += __uint_as_float(w.w & 0xffff0000u);
+            }
+            soft_sync();                                 // before the next tile's numerators take their place
             if (fail) *s_abort = 1;
             done++;
+            settle();
         }
-        if (!mbar_wait(&sm.o_done, 0u, s_abort)) fail = 55;
-        if (fail) *s_abort = 1;
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        // sums over the tokens: 32 values in 32 lanes, halved five times, lane i ends with head i
 #pragma unroll
-        for (int o = 16; o; o >>= 1)
-#pragma unroll
-            for (int i = 0; i < o; i++) {
-                const bool up = lane & o;
-                l[i] = (up ? l[i + o] : l[i]) + __shfl_xor_sync(0xffffffffu, up ? l[i] : l[i + o], o);
-            }
-        sm.part[quad][half * 32 + lane] = l[0];
-        workers_sync();
+        for (int i = 0; i < 8; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
+            if (lane < 8) sm.part[warp][8 * lane + i] = l[i];
+        }
     }
+    if (warp < AK_MMA) {
+        if (!warp_wait(&sm.o_done, 0u, s_abort)) fail = 56;
+        if (fail) *s_abort = 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
 
     const uint32_t recv = smem_u32(smem);
     // channels per receiving CTA: whole warps of 32, and the parts of all CTAs fit the panels
@@ -514,12 +604,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     __syncthreads();
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
-    if (warp < 8) {
-        const int quad = warp & 3, half = warp >> 2;
+    if (warp >= AK_SOFT && warp < AK_MMA) {
+        const int quad = warp & 3, half = (warp - AK_SOFT) >> 2;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         for (int i = 0; i < NPAIR; i++) {
-            const int ch = i * 128 + quad * 32 + lane;
-            if (ch - lane >= a.d) break;
+            const int ch0 = i * 128 + quad * 32;
+            if (ch0 >= a.d) break;
+            const bool codes = ch0 < a.d - a.rd;         // these channels lie in the order of the codes
+            const int ch = ch0 + (codes ? ak_order(lane) : lane);
             float v[32];
             if (done) {
                 uint32_t raw[32];
@@ -532,14 +624,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 for (int k = 0; k < 32; k++) v[k] = 0.f;
             }
             if (C == 1) {
-                if (!*s_abort) ak_put(a, o_at, ch, half * 32, nh, v, lane);
+                if (!*s_abort) ak_put(a, o_at, ch, codes ? 2 : 1, half * 32, nh, v);
             } else {
                 const int to = ch / slice;
                 const uint32_t base = cluster_addr(recv, to) + ((uint32_t)rank * slice + (ch - to * slice)) * (AK_HEADS * 4);
 #pragma unroll
                 for (int k = 0; k < 8; k++)
                     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(base + (((half * 8 + k) ^ (lane & 15)) << 4)), "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]),
+                                 ::"r"(base + (((half * 8 + k) ^ (ch & 15)) << 4)), "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]),
                                    "f"(v[4 * k + 3]) : "memory");
             }
         }
@@ -548,8 +640,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
         __syncwarp();
         cluster_arrive();
         cluster_wait();                                  // the parts of this CTA's channels are in; nothing remote after this
-        if (warp < 8 && !*s_abort) {
-            for (int u = warp; u < slice / 32 * 16; u += 8) {
+        if (warp < AK_MMA && !*s_abort) {
+            for (int u = warp; u < slice / 32 * 16; u += AK_MMA) {
                 const int local = (u >> 4) * 32 + lane, ch = rank * slice + local, hc = u & 15;
                 if (ch - lane >= a.d) break;
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -557,7 +649,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     const float4 x = *reinterpret_cast<const float4 *>(smem + ((size_t)r * slice + local) * (AK_HEADS * 4) + ((hc ^ (lane & 15)) << 4));
                     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
                 }
-                ak_put(a, o_at, ch, hc * 4, nh, v, lane);
+                ak_put(a, o_at, ch, 1, hc * 4, nh, v);
             }
         }
     }
