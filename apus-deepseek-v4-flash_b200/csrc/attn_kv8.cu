@@ -25,7 +25,7 @@ struct AttnKv8Args {
     int h, d, rd, idxw, rows, rows_per_seq;
     float scale;
     int q_bf16, o_bf16;
-    int cluster, unit;           // CTAs per query row, tokens per tile (a multiple of 16 up to 128)
+    int cluster, unit;           // CTAs per query row, tokens per tile (a multiple of 16 up to 112)
     int *status;
 };
 
@@ -77,31 +77,33 @@ __device__ __forceinline__ uint2 ldg8_if(const uint8_t *p, bool yes) {
 // and stays until a score exceeds it by more than 2^AK_SLACK, which in f32 and BF16, floating as both are, costs no
 // precision; only then is the accumulator scaled.  Sums of numerators stay in each thread until the end.
 //
-// A row's candidates are cut into tiles of at most 128, dealt in turn to the CTAs of a cluster.  At the end every CTA
-// tells the others its references and sums, scales its part of O^T and stores it into the shared memory of the CTA that
-// owns the channels, which adds the parts in rank order: one launch, no scratch, the same bits every time.
+// A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA
+// publishes its references and sums, scales its part of O^T and stores it into the shared memory of the CTA that owns the
+// channels, which adds the parts in rank order: one launch, no scratch, the same bits every time.
 //
-// Warps 0 to 3: queries, softmax.  Warps 4 to 11: rows, fetched into registers a tile ahead and dequantised into shared
-// memory; the output at the end.  Warp 12 issues the MMAs.  Thirteen warps have 128 registers a thread, which is what both
-// the softmax (64 sums) and the rows (72 registers in flight) need; with fewer, larger roles they spilt, and what is spilt here
-// goes to L2, since shared memory leaves no L1.  Shared memory: 8 panels of 128 tokens x 64 channels (128-byte swizzled
-// rows), Q as 8 panels of 64 heads x 64 channels, P.
-constexpr int AK_TILE = 128, AK_HEADS = 64, AK_MAX_C = 16;
-constexpr int AK_SOFT = 4, AK_ROWS = 8, AK_MMA = AK_SOFT + AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
+// Warps 0 to 3: softmax.  Warps 4 to 10: rows, fetched into registers a tile ahead and dequantised into shared memory.  Warp
+// 11 issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64
+// heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
+// shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
+// TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
+// comes of them is masked.)
+constexpr int AK_TILE = 112, AK_HEADS = 64, AK_MAX_C = 16;
+constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
-constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + AK_PANEL;
+constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
 constexpr uint32_t AK_SLACK = 40;
 constexpr float AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 
 struct AkMisc {
-    float2 ml[AK_MAX_C][AK_HEADS];                     // reference and sum of every CTA of the cluster
+    float2 ml[AK_HEADS];                                // reference and sum of this CTA
     float m[AK_HEADS], f[AK_HEADS], part[4][AK_HEADS];
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
 };
-constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc) + 1024;
-static_assert(AK_SMEM <= 227 * 1024, "shared memory of a CTA");
+constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc);
+static_assert(AK_SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
+static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32, or the parts of all CTAs, in the place of panels and queries");
 
 // barriers of the softmax warps
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -276,26 +278,19 @@ struct TileRows {
     }
 };
 
-// o[head][ch] of one warp: lane = channel ch, v[i] = head h0 + i of it, already scaled; `mate`: the lane with the other channel
-// of an even and odd pair is lane ^ mate
-template <int N>
-__device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, int mate, int h0, int nh, const float (&v)[N]) {
+// Two heads of o[head][ch]: lane = channel
+__device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, int hd, int nh, const float (&v)[2]) {
     if (!a.o_bf16) {
-        float *o = static_cast<float *>(a.o) + at + ch + (size_t)h0 * a.d;
-#pragma unroll
-        for (int i = 0; i < N; i++, o += a.d)
-            if (h0 + i < nh) *o = __uint_as_float(bf16x2_rn(v[i], 0.f) << 16);
+        float *o = static_cast<float *>(a.o) + at + (size_t)hd * a.d + ch;
+        if (hd < nh) o[0] = __uint_as_float(bf16x2_rn(v[0], 0.f) << 16);
+        if (hd + 1 < nh) o[a.d] = __uint_as_float(bf16x2_rn(v[1], 0.f) << 16);
         return;
     }
-    // the two lanes trade, so that each stores both channels of one of two heads
+    // neighbours trade, so that each stores two channels of one head
     const bool odd = ch & 1;
-    uint16_t *o = static_cast<uint16_t *>(a.o) + at + (ch & ~1) + (size_t)(h0 + odd) * a.d;
-#pragma unroll
-    for (int i = 0; i < N; i += 2, o += 2 * a.d) {
-        const float other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], mate);
-        const uint32_t w = odd ? bf16x2_rn(other, v[i + 1]) : bf16x2_rn(v[i], other);
-        if (h0 + i + odd < nh) *reinterpret_cast<uint32_t *>(o) = w;
-    }
+    const float other = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
+    const uint32_t w = odd ? bf16x2_rn(other, v[1]) : bf16x2_rn(v[0], other);
+    if (hd + odd < nh) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.o) + at + (size_t)(hd + odd) * a.d + (ch & ~1)) = w;
 }
 
 template <bool TAIL>
@@ -303,8 +298,7 @@ __global__ void __launch_bounds__(AK_THREADS, 1)
 attn_kv8_kernel(const AttnKv8Args a) {
     APUS_PDL_WAIT();
     APUS_PDL_GO();
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t smem[];
     AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + AK_MISC_OFF);
     volatile int *s_abort = &sm.abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = a.cluster;
@@ -320,7 +314,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         mbar_init(&sm.s_full, 1);
         mbar_init(&sm.p_ready, AK_SOFT);
         mbar_init(&sm.o_done, 1);
-        *s_abort = 0;
+        *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
@@ -416,7 +410,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     const uint64_t da = dv + 2 * i * (AK_PANEL >> 4);
                     ak_mma(tmem + i * AK_HEADS, da, dp, id_o, done ? 1u : 0u);
 #pragma unroll
-                    for (int k = 1; k < 8; k++)
+                    for (int k = 1; k < AK_TILE / 16; k++)
                         if (k < ks) ak_mma(tmem + i * AK_HEADS, da + 128 * k, dp + 128 * k, id_o, 1u);
                     ak_commit(&sm.empty[i]);
                 }
@@ -578,61 +572,69 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     __syncthreads();
 
-    const uint32_t recv = smem_u32(smem);
-    // channels per receiving CTA: whole warps of 32, and the parts of all CTAs fit the panels
+    // channels per receiving CTA: whole warps of 32, and the parts of all CTAs fit the place of panels and queries
     const int slice = (a.d / C + 31) & ~31;
+    if (tid < AK_HEADS) sm.ml[tid] = make_float2(sm.m[tid], (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]));
     if (C > 1) {
         cluster_wait();                                  // every CTA of the cluster has started
-        if (tid < AK_HEADS) {
-            const float sum = (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]), m = sm.m[tid];
-            for (int r = 0; r < C; r++)
-                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};"
-                             ::"r"(cluster_addr(smem_u32(&sm.ml[rank][tid]), r)), "f"(m), "f"(sum) : "memory");
-        }
         cluster_arrive();
-        cluster_wait();                                  // all references and sums are in, all panels have been read
-    } else if (tid < AK_HEADS) {
-        sm.ml[0][tid] = make_float2(sm.m[tid], (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]));
+        cluster_wait();                                  // all references and sums are there, all panels have been read
     }
     if (tid < AK_HEADS) {
-        const float sk = a.sink && tid < nh ? a.sink[h0 + tid] : -INFINITY, sk2 = sk * LOG2E;
+        const float sk2 = a.sink && tid < nh ? a.sink[h0 + tid] * LOG2E : -INFINITY;
+        float2 ml[AK_MAX_C];
+#pragma unroll
+        for (int r = 0; r < AK_MAX_C; r++) {
+            ml[r] = make_float2(AK_NONE, 0.f);
+            if (C == 1 && r == 0) ml[r] = sm.ml[tid];
+            if (C > 1 && r < C)
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                             : "=f"(ml[r].x), "=f"(ml[r].y) : "r"(cluster_addr(smem_u32(&sm.ml[tid]), r)));
+        }
         float top = fmaxf(sk2, AK_NONE);
-        for (int r = 0; r < C; r++) top = fmaxf(top, sm.ml[r][tid].x);
+#pragma unroll
+        for (int r = 0; r < AK_MAX_C; r++) top = fmaxf(top, ml[r].x);
         float den = ex2(sk2 - top);
-        for (int r = 0; r < C; r++) den += sm.ml[r][tid].y * ex2(sm.ml[r][tid].x - top);
-        sm.f[tid] = sk2 == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[rank][tid].x - top) / den;
+#pragma unroll
+        for (int r = 0; r < AK_MAX_C; r++) den += ml[r].y * ex2(ml[r].x - top);
+        sm.f[tid] = sk2 == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[tid].x - top) / den;
     }
     __syncthreads();
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
-    if (warp >= AK_SOFT && warp < AK_MMA) {
-        const int quad = warp & 3, half = (warp - AK_SOFT) >> 2;
+    if (warp < 8) {
+        const int quad = warp & 3, hh = (warp >> 2) * 32;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        float f[32];
+#pragma unroll
+        for (int k = 0; k < 32; k++) f[k] = sm.f[hh + k];
         for (int i = 0; i < NPAIR; i++) {
             const int ch0 = i * 128 + quad * 32;
             if (ch0 >= a.d) break;
-            const bool codes = ch0 < a.d - a.rd;         // these channels lie in the order of the codes
-            const int ch = ch0 + (codes ? ak_order(lane) : lane);
-            float v[32];
+            const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane);     // panels of codes have an order of their own
+            uint32_t v[32];
             if (done) {
-                uint32_t raw[32];
-                tmem_ld32(tmem + lanes + i * AK_HEADS + half * 32, raw);
+                tmem_ld32(tmem + lanes + i * AK_HEADS + hh, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = __uint_as_float(raw[k]) * sm.f[half * 32 + k];
-            } else {
-#pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = 0.f;
             }
-            if (C == 1) {
-                if (!*s_abort) ak_put(a, o_at, ch, codes ? 2 : 1, half * 32, nh, v);
-            } else {
-                const int to = ch / slice;
-                const uint32_t base = cluster_addr(recv, to) + ((uint32_t)rank * slice + (ch - to * slice)) * (AK_HEADS * 4);
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(base + (((half * 8 + k) ^ (ch & 15)) << 4)), "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]),
-                                   "f"(v[4 * k + 3]) : "memory");
+            for (int k = 0; k < 32; k++) v[k] = done ? __float_as_uint(__uint_as_float(v[k]) * f[k]) : 0u;
+            if (C > 1) {
+                // a warp's 32 channels of one head are one piece of 128 bytes (16 bytes of 32 rows took four times as long)
+                const int to = ch0 / slice;
+                const uint32_t base = cluster_addr(smem_u32(smem), to) + (((uint32_t)rank * AK_HEADS + hh) * slice + (ch - to * slice)) * 4;
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(base + k * slice * 4), "r"(v[k]) : "memory");
+            } else if (a.o_bf16) {
+                const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * 2;
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + k * a.d * 2), "h"((uint16_t)bf16x2_rn(__uint_as_float(v[k]), 0.f)));
+            } else {
+                const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * 4;
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + k * a.d * 4), "r"(bf16x2_rn(__uint_as_float(v[k]), 0.f) << 16));
             }
         }
     }
@@ -640,17 +642,26 @@ attn_kv8_kernel(const AttnKv8Args a) {
         __syncwarp();
         cluster_arrive();
         cluster_wait();                                  // the parts of this CTA's channels are in; nothing remote after this
-        if (warp < AK_MMA && !*s_abort) {
-            for (int u = warp; u < slice / 32 * 16; u += AK_MMA) {
-                const int local = (u >> 4) * 32 + lane, ch = rank * slice + local, hc = u & 15;
-                if (ch - lane >= a.d) break;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int r = 0; r < C; r++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(smem + ((size_t)r * slice + local) * (AK_HEADS * 4) + ((hc ^ (lane & 15)) << 4));
-                    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-                }
-                ak_put(a, o_at, ch, 1, hc * 4, nh, v);
+        if (!*s_abort) {
+            const float *part = reinterpret_cast<const float *>(smem) + lane;
+            const int n = min(slice, a.d - rank * slice) / 32;           // pieces of 32 channels
+            for (int u = warp; u < n * (AK_HEADS / 2); u += AK_MMA + 1) {
+                const int local = u % n * 32, hd = u / n * 2;
+                float v[2] = {0.f, 0.f};
+                for (int r = 0; r < C; r++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) v[k] += part[(size_t)(r * AK_HEADS + hd + k) * slice + local];
+                ak_put(a, o_at, rank * slice + local + lane, hd, nh, v);
             }
+        }
+    } else {
+        proxy_fence();
+        __syncthreads();
+        // the heads of this CTA are one piece of the output
+        if (tid == 0 && !*s_abort) {
+            const uint32_t bytes = (uint32_t)(nh * a.d) * (a.o_bf16 ? 2u : 4u);
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;"
+                         ::"l"(static_cast<uint8_t *>(a.o) + o_at * (a.o_bf16 ? 2 : 4)), "r"(smem_u32(smem)), "r"(bytes) : "memory");
         }
     }
     if (fail) {
@@ -674,7 +685,7 @@ void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluste
         const int k = idxw > AK_TILE * C ? (idxw + AK_TILE * C - 1) / (AK_TILE * C) : 1;      // tiles of the CTA with the most
         const int u = idxw ? ((idxw + C * k - 1) / (C * k) + 15) & ~15 : 16;
         const double waves = (double)((rows + slots[i] - 1) / slots[i]);
-        const double t = waves * (3.0 + (C > 1 ? 2.0 : 0.0) + k * (1.0 + u / 128.0 * 1.5));
+        const double t = waves * (3.0 + (C > 1 ? 2.0 : 0.0) + k * (1.0 + u / 112.0 * 1.5));
         if (i == 0 || t < best) { best = t; *cluster = C; *unit = u; }
     }
 }
