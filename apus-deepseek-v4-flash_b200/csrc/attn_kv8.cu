@@ -45,7 +45,7 @@ struct Kv8Seq {
         return reinterpret_cast<const uint8_t *>((id < na ? a : b) + (uintptr_t)(uint32_t)id * bytes);
     }
 };
-// 16 or 8 bytes of global memory, or zeros; here and not where the value is first used, and without a branch
+// 16 or 4 bytes of global memory, or zeros; here and not where the value is first used, and without a branch
 __device__ __forceinline__ uint4 ldg16_if(const uint8_t *p, bool yes) {
     uint4 v;
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
@@ -53,10 +53,10 @@ __device__ __forceinline__ uint4 ldg16_if(const uint8_t *p, bool yes) {
                  : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"((uint32_t)yes));
     return v;
 }
-__device__ __forceinline__ uint2 ldg8_if(const uint8_t *p, bool yes) {
-    uint2 v;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}"
-                 : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"((uint32_t)yes));
+__device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}"
+                 : "=&r"(v) : "l"(p), "r"((uint32_t)yes));
     return v;
 }
 
@@ -81,14 +81,15 @@ __device__ __forceinline__ uint2 ldg8_if(const uint8_t *p, bool yes) {
 // publishes its references and sums, scales its part of O^T and stores it into the shared memory of the CTA that owns the
 // channels, which adds the parts in rank order: one launch, no scratch, the same bits every time.
 //
-// Warps 0 to 3: softmax.  Warps 4 to 10: rows, fetched into registers a tile ahead and dequantised into shared memory.  Warp
-// 11 issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64
+// Warps 0 to 3: softmax.  Warps 4 to 17: rows, fetched into registers a tile ahead and dequantised into shared memory, the
+// first seven of them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one
+// dequantises.  Warp 18 issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64
 // heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
 // shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
 // TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
 // comes of them is masked.)
 constexpr int AK_TILE = 112, AK_HEADS = 64, AK_MAX_C = 16;
-constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
+constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
 constexpr uint32_t AK_SLACK = 40;
@@ -192,17 +193,12 @@ __device__ __forceinline__ uint2 codes_bf16x4(uint32_t c, uint32_t f) {
 }
 __device__ __forceinline__ int ak_order(int ch) { return (ch & ~3) | (ch & 1) << 1 | (ch >> 1 & 1); }
 // 16 codes of a group with scale byte `b` -> 16 BF16 values.  2^120 times the scale is a BF16 value up to byte 134 (rows of
-// magnitude 57,344); larger ones take two multiplications.
+// magnitude 57,344); what larger ones are above that is made up for afterwards (TileRows::enlarge).
 __device__ __forceinline__ void dequant16(const uint4 &c, uint32_t b, uint4 &lo, uint4 &hi) {
-    const uint32_t f = b <= 134u ? b * 0x00800080u + 0x3c003c00u : 0x7b807b80u;
+    const uint32_t f = min(b, 134u) * 0x00800080u + 0x3c003c00u;
     const uint2 w0 = codes_bf16x4(c.x, f), w1 = codes_bf16x4(c.y, f), w2 = codes_bf16x4(c.z, f), w3 = codes_bf16x4(c.w, f);
     lo = make_uint4(w0.x, w0.y, w1.x, w1.y);
     hi = make_uint4(w2.x, w2.y, w3.x, w3.y);
-    if (b > 134u) {
-        const uint32_t g = b == 255u ? 0x7fff7fffu : b * 0x00800080u;
-        lo = make_uint4(mul_bf16x2(lo.x, g), mul_bf16x2(lo.y, g), mul_bf16x2(lo.z, g), mul_bf16x2(lo.w, g));
-        hi = make_uint4(mul_bf16x2(hi.x, g), mul_bf16x2(hi.y, g), mul_bf16x2(hi.z, g), mul_bf16x2(hi.w, g));
-    }
 }
 // 16 bytes to shared memory.  No memory clobber: the loads that follow in the program need not wait for it (every use of what
 // is stored lies behind a fence or a barrier that has one).
@@ -225,13 +221,12 @@ struct TileIds {
     }
 };
 
-// What a lane of the row warps holds of a tile: of its rows r0 and r0 + 8, 16 channels of every panel of codes (or 16 BF16
-// values of the rotated panel, in the place of two), and the scales.
+// What a lane of the row warps holds of a tile: of its rows r0 and r0 + 8, 16 channels of each of its group's four panels, or
+// 16 BF16 values of the rotated one, and the scales of the four.
 template <bool TAIL>
 struct TileRows {
-    static constexpr int NC = TAIL ? 7 : 8;
-    uint4 c[NC][2], t[2][TAIL ? 2 : 1];
-    uint2 sc[2];
+    uint4 c[4][2], t[2][TAIL ? 2 : 1];
+    uint32_t sc[2];
     const uint8_t *rec[2];                              // of the tile that is fetched
     bool is[2];
     __device__ __forceinline__ void find(const Kv8Seq &at, const TileIds &ids, int w, int lane) {
@@ -244,36 +239,50 @@ struct TileRows {
             rec[i] = at.at(id);
         }
     }
-    __device__ __forceinline__ void load_scales(int off) {
+    // `from`: of this lane's bytes in the first panel, `np`: panels of codes and (one more) the rotated one of the group
+    __device__ __forceinline__ void load(int from, int scales, int n_codes, bool rotated, int sub) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) sc[i] = ldg8_if(rec[i] + off, is[i]);
-    }
-    // `nq`: channels held as codes
-    __device__ __forceinline__ void load(int nq, int p, bool rotated, int sub) {
+        for (int i = 0; i < 2; i++) sc[i] = ldg4_if(rec[i] + scales, is[i]);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (TAIL && rotated) {
-                t[i][0] = ldg16_if(rec[i] + nq + sub * 32, is[i]);
-                t[i][TAIL ? 1 : 0] = ldg16_if(rec[i] + nq + sub * 32 + 16, is[i]);
-            } else {
-                c[p < NC ? p : 0][i] = ldg16_if(rec[i] + p * 64 + sub * 16, is[i]);
+        for (int j = 0; j < 4; j++) {
+            if (j < n_codes) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) c[j][i] = ldg16_if(rec[i] + from + j * 64, is[i]);
+            } else if (TAIL && j == n_codes && rotated) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    t[i][0] = ldg16_if(rec[i] + from + j * 64 + sub * 16, is[i]);
+                    t[i][TAIL ? 1 : 0] = ldg16_if(rec[i] + from + j * 64 + sub * 16 + 16, is[i]);
+                }
             }
         }
     }
-    // panel p of the tile into shared memory
-    __device__ __forceinline__ void store(uint8_t *panel, int p, bool rotated, int r0, int sub) const {
+    // the group's panel j into shared memory at `at`, where this lane's part of row r0 starts; first and second half of 16
+    // channels go to x0 and x1
+    __device__ __forceinline__ void store(uint8_t *at, int j, bool codes, int x0, int x1) const {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             uint4 lo, hi;
-            if (TAIL && rotated) {
+            if (TAIL && !codes) {
                 lo = t[i][0];
                 hi = t[i][TAIL ? 1 : 0];
             } else {
-                dequant16(c[p < NC ? p : 0][i], (p < 4 ? sc[i].x >> 8 * (p & 3) : sc[i].y >> 8 * (p & 3)) & 0xffu, lo, hi);
+                dequant16(c[j][i], sc[i] >> 8 * j & 0xffu, lo, hi);
             }
-            uint8_t *row = panel + (r0 + 8 * i) * 128;
-            sts16(row + ((2 * sub) ^ (r0 & 7)) * 16, lo);
-            sts16(row + ((2 * sub + 1) ^ (r0 & 7)) * 16, hi);
+            sts16(at + i * 1024 + x0, lo);
+            sts16(at + i * 1024 + x1, hi);
+            if (codes && __any_sync(0xffffffffu, (sc[i] >> 8 * j & 0xffu) > 134u)) enlarge(at + i * 1024, sc[i] >> 8 * j & 0xffu, x0, x1);
+        }
+    }
+    // the part of a scale above byte 134, on what has been stored (255: NaN)
+    __device__ __forceinline__ static void enlarge(uint8_t *at, uint32_t b, int x0, int x1) {
+        const uint32_t g = b == 255u ? 0x7fff7fffu : (max(b, 134u) - 7u) * 0x00800080u;
+#pragma unroll 1
+        for (int k = 0; k < 8; k++) {
+            const uint32_t p = smem_u32(at + (k & 4 ? x1 : x0)) + (k & 3) * 4;
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p));
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(mul_bf16x2(v, g)));
         }
     }
 };
@@ -301,7 +310,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + AK_MISC_OFF);
     volatile int *s_abort = &sm.abort;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = a.cluster;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, C = a.cluster;
     const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * AK_HEADS, nh = min(AK_HEADS, a.h - h0);
     const long long row = blockIdx.x / (unsigned)C, seq = row / a.rows_per_seq;
     const Kv8Seq at(a, seq);
@@ -421,38 +430,42 @@ attn_kv8_kernel(const AttnKv8Args a) {
         }
         if (!fail) ak_commit(&sm.o_done);
     } else if (warp >= AK_SOFT) {
-        const int w = warp - AK_SOFT, r0 = w * 16 + (lane >> 2), sub = lane & 3;
+        const int grp = warp >= AK_SOFT + AK_ROWS, w = warp - AK_SOFT - grp * AK_ROWS, r0 = w * 16 + (lane >> 2), sub = lane & 3;
+        const int nq = a.d - a.rd;
+        // this group's panels: n of them, the last one rotated or not
+        const int n = min(max(NP - 4 * grp, 0), 4), n_codes = min(max(nq / 64 - 4 * grp, 0), 4);
+        const int from = 4 * grp * 64 + sub * 16, scales = kv8_scale_off(a.d, a.rd) + 4 * grp;
+        uint8_t *to = smem + 4 * grp * AK_PANEL + r0 * 128;
+        const int x0 = ((2 * sub) ^ (r0 & 7)) * 16, x1 = ((2 * sub + 1) ^ (r0 & 7)) * 16;
         TileRows<TAIL> rows;
-        const int nq = a.d - a.rd, scales = kv8_scale_off(a.d, a.rd);
-        auto fetch = [&]() {                             // tile `tile`, all of it
+        if (n && more) {
             rows.find(at, cur, w, lane);
-            rows.load_scales(scales);
-#pragma unroll
-            for (int p = 0; p < 8; p++)
-                if (p < NP) rows.load(nq, p, p == NP - 1, sub);
-        };
-        if (more) fetch();
+            rows.load(from, scales, n_codes, n > n_codes, sub);
+        }
         queries();
-        while (more) {
+        while (n && more) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
             cur.load(a, ids, tile, lane);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (i >= NPAIR) break;
-                if (!warp_wait(&sm.empty[i], (done & 1u) ^ 1u, s_abort)) fail = 54;
-                if (r0 < held) {
+            for (int i = 0; i < 2; i++) {
+                if (2 * i >= n) break;
+                if (!warp_wait(&sm.empty[2 * grp + i], (done & 1u) ^ 1u, s_abort)) fail = 54;
+                if (w * 16 < held) {
 #pragma unroll
-                    for (int p = 2 * i; p < 2 * i + 2; p++)
-                        if (p < NP) rows.store(smem + p * AK_PANEL, p, p == NP - 1, r0, sub);
+                    for (int j = 2 * i; j < 2 * i + 2; j++)
+                        if (j < n) rows.store(to + j * AK_PANEL, j, j < n_codes, x0, x1);
                 }
                 proxy_fence();
-                mbar_arrive_warp(&sm.full[i], lane);
+                mbar_arrive_warp(&sm.full[2 * grp + i], lane);
             }
-            // The next tile's rows, all at once: they have the softmax and the first MMAs on the values to arrive.  Loads issued
-            // between the stores above would be waited for there, since a thread has few counters of loads in flight.
+            // The next tile's rows, all at once: they have the rest of this tile to arrive.  Loads issued between the stores
+            // above would be waited for there, since a thread has few counters of loads in flight.
             settle();
-            if (more) fetch();
+            if (more) {
+                rows.find(at, cur, w, lane);
+                rows.load(from, scales, n_codes, n > n_codes, sub);
+            }
             if (fail) *s_abort = 1;
             done++;
         }
