@@ -92,12 +92,14 @@ constexpr int AK_TILE = 112, AK_HEADS = 64, AK_MAX_C = 16;
 constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
-constexpr uint32_t AK_SLACK = 40;
+constexpr uint32_t AK_SLACK = 64;
 constexpr float AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 
 struct AkMisc {
     float2 ml[AK_HEADS];                                // reference and sum of this CTA
-    float m[AK_HEADS], f[AK_HEADS], part[4][AK_HEADS];
+    alignas(16) float m[AK_HEADS];
+    alignas(16) float f[AK_HEADS];
+    float part[4][AK_HEADS], sink[AK_HEADS];            // sinks times log2 e
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
@@ -131,9 +133,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float redux_max(float x) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -194,7 +196,7 @@ __device__ __forceinline__ uint2 codes_bf16x4(uint32_t c, uint32_t f) {
 __device__ __forceinline__ int ak_order(int ch) { return (ch & ~3) | (ch & 1) << 1 | (ch >> 1 & 1); }
 // 16 codes of a group with scale byte `b` -> 16 BF16 values.  2^120 times the scale is a BF16 value up to byte 134 (rows of
 // magnitude 57,344); what larger ones are above that is made up for afterwards (TileRows::enlarge).
-__device__ __forceinline__ void dequant16(const uint4 &c, uint32_t b, uint4 &lo, uint4 &hi) {
+__device__ __forceinline__ void dequant16(const uint4 c, uint32_t b, uint4 &lo, uint4 &hi) {
     const uint32_t f = min(b, 134u) * 0x00800080u + 0x3c003c00u;
     const uint2 w0 = codes_bf16x4(c.x, f), w1 = codes_bf16x4(c.y, f), w2 = codes_bf16x4(c.z, f), w3 = codes_bf16x4(c.w, f);
     lo = make_uint4(w0.x, w0.y, w1.x, w1.y);
@@ -221,68 +223,65 @@ struct TileIds {
     }
 };
 
-// What a lane of the row warps holds of a tile: of its rows r0 and r0 + 8, 16 channels of each of its group's four panels, or
-// 16 BF16 values of the rotated one, and the scales of the four.
+// What a lane of the row warps holds of a tile: of its rows r0 and r0 + 8, 16 channels of each of its group's four panels, as
+// they were fetched (codes in the first half of v, or the BF16 values of the rotated panel) and then as BF16 values.
 template <bool TAIL>
 struct TileRows {
-    uint4 c[4][2], t[2][TAIL ? 2 : 1];
+    uint4 v[4][2][2];                                   // panel, row, half
     uint32_t sc[2];
-    const uint8_t *rec[2];                              // of the tile that is fetched
-    bool is[2];
-    __device__ __forceinline__ void find(const Kv8Seq &at, const TileIds &ids, int w, int lane) {
-        const int src = (w & 1) * 16 + (lane >> 2);
+    // `from`: of this lane's bytes in the group's first panel; the first n_codes panels hold codes, the n-th may be rotated
+    __device__ __forceinline__ void load(const Kv8Seq &at, const TileIds &ids, int w, int lane, int from, int scales, int n_codes, int n) {
+        const int src = (w & 1) * 16 + (lane >> 2), sub = lane & 3;
         const int mine = w >> 1 == 0 ? ids.id[0] : w >> 1 == 1 ? ids.id[1] : w >> 1 == 2 ? ids.id[2] : ids.id[3];
+        const uint8_t *rec[2];
+        bool is[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int id = __shfl_sync(0xffffffffu, mine, src + 8 * i);
             is[i] = id >= 0;
             rec[i] = at.at(id);
+            sc[i] = ldg4_if(rec[i] + scales, is[i]);
         }
-    }
-    // `from`: of this lane's bytes in the first panel, `np`: panels of codes and (one more) the rotated one of the group
-    __device__ __forceinline__ void load(int from, int scales, int n_codes, bool rotated, int sub) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) sc[i] = ldg4_if(rec[i] + scales, is[i]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j < n_codes) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) c[j][i] = ldg16_if(rec[i] + from + j * 64, is[i]);
-            } else if (TAIL && j == n_codes && rotated) {
+                for (int i = 0; i < 2; i++) v[j][i][0] = ldg16_if(rec[i] + from + j * 64, is[i]);
+            } else if (TAIL && j < n) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    t[i][0] = ldg16_if(rec[i] + from + j * 64 + sub * 16, is[i]);
-                    t[i][TAIL ? 1 : 0] = ldg16_if(rec[i] + from + j * 64 + sub * 16 + 16, is[i]);
+                    v[j][i][0] = ldg16_if(rec[i] + from + j * 64 + sub * 16, is[i]);
+                    v[j][i][1] = ldg16_if(rec[i] + from + j * 64 + sub * 16 + 16, is[i]);
                 }
             }
         }
     }
-    // the group's panel j into shared memory at `at`, where this lane's part of row r0 starts; first and second half of 16
-    // channels go to x0 and x1
-    __device__ __forceinline__ void store(uint8_t *at, int j, bool codes, int x0, int x1) const {
+    __device__ __forceinline__ void convert(int n_codes) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < n_codes)
+#pragma unroll
+                for (int i = 0; i < 2; i++) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
+    }
+    // the group's panel j into shared memory at `to`, where this lane's part of row r0 starts; the halves of its 16 channels
+    // go to x0 and x1
+    __device__ __forceinline__ void store(uint8_t *to, int j, bool codes, int x0, int x1) const {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            uint4 lo, hi;
-            if (TAIL && !codes) {
-                lo = t[i][0];
-                hi = t[i][TAIL ? 1 : 0];
-            } else {
-                dequant16(c[j][i], sc[i] >> 8 * j & 0xffu, lo, hi);
-            }
-            sts16(at + i * 1024 + x0, lo);
-            sts16(at + i * 1024 + x1, hi);
-            if (codes && __any_sync(0xffffffffu, (sc[i] >> 8 * j & 0xffu) > 134u)) enlarge(at + i * 1024, sc[i] >> 8 * j & 0xffu, x0, x1);
+            sts16(to + i * 1024 + x0, v[j][i][0]);
+            sts16(to + i * 1024 + x1, v[j][i][1]);
+            if (codes && __any_sync(0xffffffffu, (sc[i] >> 8 * j & 0xffu) > 134u)) enlarge(to + i * 1024, sc[i] >> 8 * j & 0xffu, x0, x1);
         }
     }
     // the part of a scale above byte 134, on what has been stored (255: NaN)
-    __device__ __forceinline__ static void enlarge(uint8_t *at, uint32_t b, int x0, int x1) {
+    __device__ __forceinline__ static void enlarge(uint8_t *to, uint32_t b, int x0, int x1) {
         const uint32_t g = b == 255u ? 0x7fff7fffu : (max(b, 134u) - 7u) * 0x00800080u;
 #pragma unroll 1
         for (int k = 0; k < 8; k++) {
-            const uint32_t p = smem_u32(at + (k & 4 ? x1 : x0)) + (k & 3) * 4;
-            uint32_t v;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p));
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(mul_bf16x2(v, g)));
+            const uint32_t p = smem_u32(to + (k & 4 ? x1 : x0)) + (k & 3) * 4;
+            uint32_t u;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(p));
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(mul_bf16x2(u, g)));
         }
     }
 };
@@ -326,7 +325,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
         *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
+    if (tid < AK_HEADS) {
+        sm.m[tid] = AK_NONE;
+        sm.sink[tid] = a.sink && tid < nh ? a.sink[h0 + tid] * LOG2E : -INFINITY;
+    }
     if (warp == AK_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
@@ -354,6 +356,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     };
     cur.load(a, ids, tile, lane);
     settle();
+    const bool any = more;                               // there is an output to read
 
     // the queries into shared memory, 8 channels at a time, by all warps but the one of the MMAs
     auto queries = [&]() {
@@ -438,15 +441,13 @@ attn_kv8_kernel(const AttnKv8Args a) {
         uint8_t *to = smem + 4 * grp * AK_PANEL + r0 * 128;
         const int x0 = ((2 * sub) ^ (r0 & 7)) * 16, x1 = ((2 * sub + 1) ^ (r0 & 7)) * 16;
         TileRows<TAIL> rows;
-        if (n && more) {
-            rows.find(at, cur, w, lane);
-            rows.load(from, scales, n_codes, n > n_codes, sub);
-        }
+        if (n && more) rows.load(at, cur, w, lane, from, scales, n_codes, n);
         queries();
         while (n && more) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
             cur.load(a, ids, tile, lane);
+            rows.convert(n_codes);                       // before there is room for it, while the tile before is worked on
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (2 * i >= n) break;
@@ -459,13 +460,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 proxy_fence();
                 mbar_arrive_warp(&sm.full[2 * grp + i], lane);
             }
-            // The next tile's rows, all at once: they have the rest of this tile to arrive.  Loads issued between the stores
-            // above would be waited for there, since a thread has few counters of loads in flight.
+            // The next tile's rows, all at once: between the stores above their issue would hold up the second one, and the MMAs
+            // that wait for it.
             settle();
-            if (more) {
-                rows.find(at, cur, w, lane);
-                rows.load(from, scales, n_codes, n > n_codes, sub);
-            }
+            if (more) rows.load(at, cur, w, lane, from, scales, n_codes, n);
             if (fail) *s_abort = 1;
             done++;
         }
@@ -490,20 +488,29 @@ attn_kv8_kernel(const AttnKv8Args a) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (bool set = done == 0;; set = true) {
                 if (set) {
-                    // new references: the maxima over the tokens so far
+                    // New references: the maxima over the tokens so far, as BF16 (they need not be exact), two heads in a register
+                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1.
+                    uint32_t x[32];
 #pragma unroll
                     for (int hf = 0; hf < 2; hf++) {
                         uint32_t s[32];
                         tmem_ld32(tmem_s + lanes + 32 * hf, s);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        float keep = AK_NONE;
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float r = redux_max(valid ? __uint_as_float(s[i]) * cs : -INFINITY);
-                            if (lane == i) keep = r;
+                        for (int i = 0; i < 16; i++) {
+                            const uint32_t u = bf16x2_rn(__uint_as_float(s[2 * i]) * cs, __uint_as_float(s[2 * i + 1]) * cs);
+                            x[16 * hf + i] = (u & mask) | (0xff80ff80u & ~mask);
                         }
-                        sm.part[warp][32 * hf + lane] = keep;
                     }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < o; i++) {
+                            const bool up = lane & o;
+                            x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
+                        }
+                    sm.part[warp][2 * lane] = __uint_as_float(x[0] << 16);
+                    sm.part[warp][2 * lane + 1] = __uint_as_float(x[0] & 0xffff0000u);
                     soft_sync();
                     if (tid < AK_HEADS) {
                         const float old = sm.m[tid];
@@ -515,13 +522,20 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     if (done) {
 #pragma unroll
                         for (int i = 0; i < 8; i++) l[i] *= sm.f[8 * lh + i];
-                        for (int i = 0; i < 2 * NPAIR; i++) {
-                            uint32_t v[32];
-                            tmem_ld32(tmem + lanes + 32 * i, v);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll 1
+                        for (int hf = 0; hf < 2; hf++) {
+                            float f[32];
 #pragma unroll
-                            for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * sm.f[32 * (i & 1) + k]);
-                            tmem_st32(tmem + lanes + 32 * i, v);
+                            for (int k = 0; k < 32; k++) f[k] = sm.f[32 * hf + k];
+#pragma unroll 1
+                            for (int i = 0; i < NPAIR; i++) {
+                                uint32_t v[32];
+                                tmem_ld32(tmem + lanes + i * AK_HEADS + 32 * hf, v);
+                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * f[k]);
+                                tmem_st32(tmem + lanes + i * AK_HEADS + 32 * hf, v);
+                            }
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
@@ -594,13 +608,12 @@ attn_kv8_kernel(const AttnKv8Args a) {
         cluster_wait();                                  // all references and sums are there, all panels have been read
     }
     if (tid < AK_HEADS) {
-        const float sk2 = a.sink && tid < nh ? a.sink[h0 + tid] * LOG2E : -INFINITY;
+        const float sk2 = sm.sink[tid];
         float2 ml[AK_MAX_C];
 #pragma unroll
         for (int r = 0; r < AK_MAX_C; r++) {
             ml[r] = make_float2(AK_NONE, 0.f);
-            if (C == 1 && r == 0) ml[r] = sm.ml[tid];
-            if (C > 1 && r < C)
+            if (r == 0 || r < C)
                 asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
                              : "=f"(ml[r].x), "=f"(ml[r].y) : "r"(cluster_addr(smem_u32(&sm.ml[tid]), r)));
         }
@@ -609,28 +622,29 @@ attn_kv8_kernel(const AttnKv8Args a) {
         for (int r = 0; r < AK_MAX_C; r++) top = fmaxf(top, ml[r].x);
         float den = ex2(sk2 - top);
 #pragma unroll
-        for (int r = 0; r < AK_MAX_C; r++) den += ml[r].y * ex2(ml[r].x - top);
+        for (int r = 0; r < AK_MAX_C; r++)
+            if (r == 0 || r < C) den += ml[r].y * ex2(ml[r].x - top);
         sm.f[tid] = sk2 == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[tid].x - top) / den;
     }
     __syncthreads();
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
-    if (warp < 8) {
-        const int quad = warp & 3, hh = (warp >> 2) * 32;
+    if (warp < 16) {
+        const int quad = warp & 3, hh = (warp >> 2 & 1) * 32;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         float f[32];
 #pragma unroll
         for (int k = 0; k < 32; k++) f[k] = sm.f[hh + k];
-        for (int i = 0; i < NPAIR; i++) {
+        for (int i = warp >> 3; i < NPAIR; i += 2) {
             const int ch0 = i * 128 + quad * 32;
             if (ch0 >= a.d) break;
             const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane);     // panels of codes have an order of their own
             uint32_t v[32];
-            if (done) {
+            if (any) {
                 tmem_ld32(tmem + lanes + i * AK_HEADS + hh, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             }
 #pragma unroll
-            for (int k = 0; k < 32; k++) v[k] = done ? __float_as_uint(__uint_as_float(v[k]) * f[k]) : 0u;
+            for (int k = 0; k < 32; k++) v[k] = any ? __float_as_uint(__uint_as_float(v[k]) * f[k]) : 0u;
             if (C > 1) {
                 // a warp's 32 channels of one head are one piece of 128 bytes (16 bytes of 32 rows took four times as long)
                 const int to = ch0 / slice;
