@@ -138,11 +138,6 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -186,18 +181,12 @@ __device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr) {
            (uint64_t)2 << 61;
 }
 
-// Four codes -> four BF16 values in the order 0 2 | 1 3, times 2^120 the factor in `f` (a BF16 value twice).  Exponent and
-// significand move to their places in BF16 (whose bias is 120 larger; a subnormal code becomes a subnormal value) and the
-// sign goes into the factor.  The order saves the byte permutations: integer instructions issue every other cycle, and they
-// bound this (64 codes of a lane: 330 -> 200 cycles of a scheduler).  Queries and output channels follow it (ak_order).
-__device__ __forceinline__ uint2 codes_bf16x4(uint32_t c, uint32_t f) {
-    return make_uint2(mul_bf16x2(c << 4 & 0x07f007f0u, (c << 8 & 0x80008000u) | f), mul_bf16x2(c >> 4 & 0x07f007f0u, (c & 0x80008000u) | f));
-}
+// Where a channel of a panel of codes lies (codes_bf16x4): queries and output channels follow it.
 __device__ __forceinline__ int ak_order(int ch) { return (ch & ~3) | (ch & 1) << 1 | (ch >> 1 & 1); }
 // 16 codes of a group with scale byte `b` -> 16 BF16 values.  2^120 times the scale is a BF16 value up to byte 134 (rows of
 // magnitude 57,344); what larger ones are above that is made up for afterwards (TileRows::enlarge).
 __device__ __forceinline__ void dequant16(const uint4 c, uint32_t b, uint4 &lo, uint4 &hi) {
-    const uint32_t f = min(b, 134u) * 0x00800080u + 0x3c003c00u;
+    const uint32_t f = code_factor(min(b, 134u));
     const uint2 w0 = codes_bf16x4(c.x, f), w1 = codes_bf16x4(c.y, f), w2 = codes_bf16x4(c.z, f), w3 = codes_bf16x4(c.w, f);
     lo = make_uint4(w0.x, w0.y, w1.x, w1.y);
     hi = make_uint4(w2.x, w2.y, w3.x, w3.y);

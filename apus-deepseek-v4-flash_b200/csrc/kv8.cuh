@@ -27,6 +27,20 @@ __device__ __forceinline__ float kv8_scale(uint32_t b) {
     return b == 255u ? __uint_as_float(0x7fffffffu) : ue8m0_f32(b);
 }
 
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Four codes -> four BF16 values in the order 0 2 | 1 3, times 2^-120 and the factor in `f` (a BF16 value twice).  Exponent
+// and significand move to their places in BF16 (whose bias is 120 larger; a subnormal code becomes a subnormal value) and
+// the sign goes into the factor.  The order saves the byte permutations: integer instructions issue every other cycle, and
+// they bound this.
+__device__ __forceinline__ uint2 codes_bf16x4(uint32_t c, uint32_t f) {
+    return make_uint2(mul_bf16x2(c << 4 & 0x07f007f0u, (c << 8 & 0x80008000u) | f), mul_bf16x2(c >> 4 & 0x07f007f0u, (c & 0x80008000u) | f));
+}
+// 2^120 times the scale of byte b <= 134, twice
+__device__ __forceinline__ uint32_t code_factor(uint32_t b) { return b * 0x00800080u + 0x3c003c00u; }
 // Two f32 -> two BF16, nearest even, lo in the low half; a NaN stays one whatever its payload is.
 __device__ __forceinline__ uint32_t bf16x2_rn(float lo, float hi) {
     uint32_t r;

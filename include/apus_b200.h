@@ -520,9 +520,10 @@ int apus_cuda_sparse_attn_batch_dev(const float *q, const float *sink, int h, in
  * of 64 with an infinity or a NaN in it reads back as NaN.  d: a multiple of 64 up to 512; rd: 0
  * or 64, below d (0 bytes and a message otherwise).
  * A cache is the caller's device memory: n_seq sequences of `cap` records, sequence b from record
- * b * stride on.  All pointers are device pointers and start on 16-byte boundaries (pos, counts,
- * idx, idxs and sink on their types'); work is enqueued on `stream`, nothing is kept between
- * calls and no memory is allocated, so calls may run side by side and be recorded into graphs. */
+ * b * stride on.  All pointers are device pointers; caches, queries and outputs start on 16-byte
+ * boundaries, f32 rows that are written or read on 32-byte ones.  Work is enqueued on `stream`,
+ * nothing is kept between calls and no memory is allocated, so calls may run side by side and be
+ * recorded into graphs. */
 size_t apus_cuda_kv8_row_bytes(int d, int rd);
 /* Quantises x [n_seq, s, d] (f32, or BF16 when x_bf16) into the caches: row t of sequence b goes to
  * entry pos[b] + t (pos [n_seq], on the device), modulo cap when `ring`.  counts [n_seq]

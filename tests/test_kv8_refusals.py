@@ -32,7 +32,7 @@ def test_row_bytes():
 
 @pytest.mark.parametrize("change,word", [
     (dict(n_seq=-1), "sequences"), (dict(s=-1), "sequences"), (dict(cap=-1), "cap"), (dict(stride=-1), "stride"), (dict(stride=127), "apart"),
-    (dict(cache=None), "no cache"), (dict(cache=CACHE + 8), "16-byte"), (dict(x=None), "rows"), (dict(x=X + 4), "16-byte"),
+    (dict(cache=None), "no cache"), (dict(cache=CACHE + 8), "16-byte"), (dict(x=None), "rows"), (dict(x=X + 16), "32-byte"), (dict(x=X + 4, bf16=1), "16-byte"),
     (dict(pos=None), "positions"), (dict(n_seq=1 << 20, s=1 << 20), "too many")])
 def test_write(change, word):
     refused("apus_cuda_kv8_write_dev", WRITE, change, word)
@@ -40,7 +40,7 @@ def test_write(change, word):
 
 @pytest.mark.parametrize("change,word", [
     (dict(n_seq=-1), "sequences"), (dict(cap=-1), "cap"), (dict(stride=-2), "stride"), (dict(cache=None), "no cache"), (dict(cache=CACHE + 1), "16-byte"),
-    (dict(out=None), "output"), (dict(out=OUT + 4), "output"), (dict(n_seq=1 << 20, s=1 << 20), "too many")])
+    (dict(out=None), "output"), (dict(out=OUT + 16), "32-byte"), (dict(out=OUT + 4, bf16=1), "16-byte"), (dict(n_seq=1 << 20, s=1 << 20), "too many")])
 def test_read(change, word):
     refused("apus_cuda_kv8_read_dev", READ, change, word)
 
