@@ -88,7 +88,7 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
 // TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
 // comes of them is masked.)
-constexpr int AK_TILE = 112, AK_HEADS = 64, AK_MAX_C = 16;
+constexpr int AK_TILE = 112, AK_HEADS = 64;
 constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
@@ -99,7 +99,7 @@ struct AkMisc {
     float2 ml[AK_HEADS];                                // reference and sum of this CTA
     alignas(16) float m[AK_HEADS];
     alignas(16) float f[AK_HEADS];
-    float part[4][AK_HEADS], sink[AK_HEADS];            // sinks times log2 e
+    float part[4][AK_HEADS];
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
@@ -123,9 +123,24 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-// A wait of a whole warp, which goes on together
+// A wait of a whole warp, which goes on together; false when it ran out or another one did.  One loop, not unrolled, like the
+// others below: this kernel's roles run through their code once per tile, and what the instruction caches do not hold they
+// wait for (124 KB of code, half of it unrolled waits, took 20 % longer than 60 KB).
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+    const uint32_t addr = smem_u32(bar);
+    unsigned long long t0 = 0;
+    uint32_t ok = 0;
+#pragma unroll 1
+    for (uint32_t it = 1; !ok; it++) {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
+        if (!ok && (it & 255u) == 0u) {
+            const unsigned long long now = global_ns();
+            if (!t0) t0 = now;
+            if (*abort_flag || now - t0 > TC_WAIT_BUDGET_NS) break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -252,25 +267,30 @@ struct TileRows {
 #pragma unroll
                 for (int i = 0; i < 2; i++) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
     }
-    // the group's panel j into shared memory at `to`, where this lane's part of row r0 starts; the halves of its 16 channels
-    // go to x0 and x1
-    __device__ __forceinline__ void store(uint8_t *to, int j, bool codes, int x0, int x1) const {
+    // panels 2 i2 and 2 i2 + 1 of the group's n into shared memory; `to`: where this lane's part of row r0 starts in the group's
+    // first panel; the halves of its 16 channels go to x0 and x1
+    __device__ __forceinline__ void store(uint8_t *to, int i2, int n, int n_codes, int x0, int x1) const {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            sts16(to + i * 1024 + x0, v[j][i][0]);
-            sts16(to + i * 1024 + x1, v[j][i][1]);
-            if (codes && __any_sync(0xffffffffu, (sc[i] >> 8 * j & 0xffu) > 134u)) enlarge(to + i * 1024, sc[i] >> 8 * j & 0xffu, x0, x1);
-        }
-    }
-    // the part of a scale above byte 134, on what has been stored (255: NaN)
-    __device__ __forceinline__ static void enlarge(uint8_t *to, uint32_t b, int x0, int x1) {
-        const uint32_t g = b == 255u ? 0x7fff7fffu : (max(b, 134u) - 7u) * 0x00800080u;
+        for (int j = 2 * i2; j < 2 * i2 + 2; j++)
+            if (j < n)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    sts16(to + j * AK_PANEL + i * 1024 + x0, v[j][i][0]);
+                    sts16(to + j * AK_PANEL + i * 1024 + x1, v[j][i][1]);
+                }
+        // the part of a scale above byte 134, on what has been stored (255: NaN)
+        const uint32_t top = max_u16x2(max_u16x2(sc[0] & 0x00ff00ffu, sc[0] >> 8 & 0x00ff00ffu), max_u16x2(sc[1] & 0x00ff00ffu, sc[1] >> 8 & 0x00ff00ffu));
+        if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > 134u)) {
 #pragma unroll 1
-        for (int k = 0; k < 8; k++) {
-            const uint32_t p = smem_u32(to + (k & 4 ? x1 : x0)) + (k & 3) * 4;
-            uint32_t u;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(p));
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(mul_bf16x2(u, g)));
+            for (int k = 0; k < 32; k++) {
+                const int j = 2 * i2 + (k >> 4), i = k >> 3 & 1;
+                const uint32_t b = (i ? sc[1] : sc[0]) >> 8 * j & 0xffu, p = smem_u32(to + j * AK_PANEL + i * 1024 + (k & 4 ? x1 : x0)) + (k & 3) * 4;
+                if (j < n_codes && b > 134u) {
+                    uint32_t u;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u) : "r"(p));
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(p), "r"(mul_bf16x2(u, b == 255u ? 0x7fff7fffu : (b - 7u) * 0x00800080u)));
+                }
+            }
         }
     }
 };
@@ -300,10 +320,51 @@ attn_kv8_kernel(const AttnKv8Args a) {
     volatile int *s_abort = &sm.abort;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, C = a.cluster;
     const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * AK_HEADS, nh = min(AK_HEADS, a.h - h0);
-    const long long row = blockIdx.x / (unsigned)C, seq = row / a.rows_per_seq;
+    const uint32_t row = blockIdx.x / (unsigned)C, seq = row / (uint32_t)a.rows_per_seq;
     const Kv8Seq at(a, seq);
     const int32_t *ids = a.idxs + (size_t)row * a.idxw;
     const int n_tiles = (a.idxw + a.unit - 1) / a.unit, NP = a.d / 64, NPAIR = (NP + 1) / 2;
+
+    // What the first tile waits for is asked for before anything else: its ids, sinks, and the queries, 8 channels at a time,
+    // four times at once, by all warps but the one of the MMAs
+    TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
+    int tile = rank;
+    cur.load(a, ids, tile, lane);
+    uint4 qv[4][2];
+    const int per_head = a.d / 8, q_heads = 32 * AK_MMA / per_head, q_rest = 32 * AK_MMA % per_head;
+    int q_head = tid / per_head, q_c = tid % per_head;   // of this thread's next piece
+    auto ask = [&]() {
+        const uint8_t *q = static_cast<const uint8_t *>(a.q) + ((size_t)row * a.h + h0) * a.d * (a.q_bf16 ? 2 : 4);
+        int hd = q_head, c = q_c;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint8_t *p = q + (uint32_t)(hd < nh ? hd * per_head + c : 0) * (a.q_bf16 ? 16u : 32u);
+            qv[k][0] = ldg16_if(p, hd < nh);
+            qv[k][1] = ldg16_if(p + 16, hd < nh && !a.q_bf16);
+            hd += q_heads;
+            c += q_rest;
+            if (c >= per_head) { c -= per_head; hd++; }
+        }
+    };
+    auto place = [&]() {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint4 v = qv[k][0];
+            if (!a.q_bf16)
+                v = make_uint4(bf16x2_rn(__uint_as_float(v.x), __uint_as_float(v.y)), bf16x2_rn(__uint_as_float(v.z), __uint_as_float(v.w)),
+                               bf16x2_rn(__uint_as_float(qv[k][1].x), __uint_as_float(qv[k][1].y)),
+                               bf16x2_rn(__uint_as_float(qv[k][1].z), __uint_as_float(qv[k][1].w)));
+            if (q_c * 8 < a.d - a.rd)                    // in the order of the codes
+                v = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x5410),
+                               __byte_perm(v.z, v.w, 0x7632));
+            if (q_head < AK_HEADS) sts16(smem + AK_Q_OFF + (q_c >> 3) * AK_QPANEL + q_head * 128 + (((q_c & 7) ^ (q_head & 7)) << 4), v);
+            q_head += q_heads;
+            q_c += q_rest;
+            if (q_c >= per_head) { q_c -= per_head; q_head++; }
+        }
+    };
+    if (warp != AK_MMA) ask();
+    const float sink = a.sink && tid < nh ? a.sink[h0 + tid] : -INFINITY;        // of head tid
 
     if (tid == 0) {
         for (int i = 0; i < 4; i++) { mbar_init(&sm.full[i], AK_ROWS); mbar_init(&sm.empty[i], 1); }
@@ -314,10 +375,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < AK_HEADS) {
-        sm.m[tid] = AK_NONE;
-        sm.sink[tid] = a.sink && tid < nh ? a.sink[h0 + tid] * LOG2E : -INFINITY;
-    }
+    if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
     if (warp == AK_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
@@ -333,52 +391,25 @@ attn_kv8_kernel(const AttnKv8Args a) {
     // through all the same, so that no thread is left waiting, and nothing is written.
     int fail = 0;
     uint32_t done = 0;                                   // tiles of this CTA so far
-    TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
-    int tile = rank;
     bool more = false;
     auto settle = [&]() {                                // cur has been asked for: the first tile from it on with a record
+#pragma unroll 1
         for (more = false; tile < n_tiles; ) {
             if ((more = cur.any(at.n))) break;
             tile += C;
             cur.load(a, ids, tile, lane);
         }
     };
-    cur.load(a, ids, tile, lane);
     settle();
     const bool any = more;                               // there is an output to read
 
-    // the queries into shared memory, 8 channels at a time, by all warps but the one of the MMAs
-    auto queries = [&]() {
-        const int per_head = a.d / 8, n = AK_HEADS * per_head, step = 32 * AK_MMA;
-        for (int i0 = tid; i0 < n; i0 += 4 * step) {
-            uint4 v[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * step, head = i / per_head;
-                const bool there = i < n && head < nh;
-                const size_t from = ((size_t)row * a.h + h0) * a.d + (there ? i : 0) * 8;
-                if (a.q_bf16) {
-                    v[k] = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 2, there);
-                } else {
-                    const uint4 x = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 4, there);
-                    const uint4 y = ldg16_if(reinterpret_cast<const uint8_t *>(a.q) + from * 4 + 16, there);
-                    v[k] = make_uint4(bf16x2_rn(__uint_as_float(x.x), __uint_as_float(x.y)), bf16x2_rn(__uint_as_float(x.z), __uint_as_float(x.w)),
-                                      bf16x2_rn(__uint_as_float(y.x), __uint_as_float(y.y)), bf16x2_rn(__uint_as_float(y.z), __uint_as_float(y.w)));
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int i = i0 + k * step, head = i / per_head, c = i - head * per_head;
-                if (c * 8 < a.d - a.rd)                  // in the order of the codes
-                    v[k] = make_uint4(__byte_perm(v[k].x, v[k].y, 0x5410), __byte_perm(v[k].x, v[k].y, 0x7632),
-                                      __byte_perm(v[k].z, v[k].w, 0x5410), __byte_perm(v[k].z, v[k].w, 0x7632));
-                if (i < n) sts16(smem + AK_Q_OFF + (c >> 3) * AK_QPANEL + head * 128 + (((c & 7) ^ (head & 7)) << 4), v[k]);
-            }
-        }
+    if (warp != AK_MMA) place();
+    auto queries = [&]() {                               // the rest of them
+#pragma unroll 1
+        while (__any_sync(0xffffffffu, q_head < AK_HEADS)) { ask(); place(); }
         proxy_fence();
         mbar_arrive_warp(&sm.q_full, lane);
     };
-
     if (warp == AK_MMA) {
         const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
         const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
@@ -388,26 +419,23 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const int ks = (min(a.unit, a.idxw - tile * a.unit) + 15) >> 4;      // steps of 16 tokens that hold any
             tile += C;
             cur.load(a, ids, tile, lane);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (i >= NPAIR || fail) break;
-                if (!warp_wait(&sm.full[i], done & 1u, s_abort)) { fail = 52; break; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int pn = 2 * i; pn < 2 * i + 2; pn++) {
-                    if (pn >= NP) break;
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        ak_mma(tmem_s, dk + pn * (AK_PANEL >> 4) + 2 * j, dq + pn * (AK_QPANEL >> 4) + 2 * j, id_s, (pn | j) ? 1u : 0u);
+#pragma unroll 1
+            for (int pn = 0; pn < NP && !fail; pn++) {
+                if (!(pn & 1)) {
+                    if (!warp_wait(&sm.full[pn >> 1], done & 1u, s_abort)) fail = 52;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
+                const uint64_t da = dk + pn * (AK_PANEL >> 4), db = dq + pn * (AK_QPANEL >> 4);
+                if (!fail)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ak_mma(tmem_s, da + 2 * j, db + 2 * j, id_s, (pn | j) ? 1u : 0u);
             }
             if (!fail) ak_commit(&sm.s_full);
             if (!fail && !warp_wait(&sm.p_ready, done & 1u, s_abort)) fail = 53;
             if (!fail) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (i >= NPAIR) break;
+#pragma unroll 1
+                for (int i = 0; i < NPAIR; i++) {
                     const uint64_t da = dv + 2 * i * (AK_PANEL >> 4);
                     ak_mma(tmem + i * AK_HEADS, da, dp, id_o, done ? 1u : 0u);
 #pragma unroll
@@ -441,11 +469,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
             for (int i = 0; i < 2; i++) {
                 if (2 * i >= n) break;
                 if (!warp_wait(&sm.empty[2 * grp + i], (done & 1u) ^ 1u, s_abort)) fail = 54;
-                if (w * 16 < held) {
-#pragma unroll
-                    for (int j = 2 * i; j < 2 * i + 2; j++)
-                        if (j < n) rows.store(to + j * AK_PANEL, j, j < n_codes, x0, x1);
-                }
+                if (w * 16 < held) rows.store(to, i, n, n_codes, x0, x1);
                 proxy_fence();
                 mbar_arrive_warp(&sm.full[2 * grp + i], lane);
             }
@@ -478,28 +502,30 @@ attn_kv8_kernel(const AttnKv8Args a) {
             for (bool set = done == 0;; set = true) {
                 if (set) {
                     // New references: the maxima over the tokens so far, as BF16 (they need not be exact), two heads in a register
-                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1.
-                    uint32_t x[32];
-#pragma unroll
+                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1 of a half.
+#pragma unroll 1
                     for (int hf = 0; hf < 2; hf++) {
-                        uint32_t s[32];
+                        uint32_t s[32], x[16];
                         tmem_ld32(tmem_s + lanes + 32 * hf, s);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             const uint32_t u = bf16x2_rn(__uint_as_float(s[2 * i]) * cs, __uint_as_float(s[2 * i + 1]) * cs);
-                            x[16 * hf + i] = (u & mask) | (0xff80ff80u & ~mask);
+                            x[i] = (u & mask) | (0xff80ff80u & ~mask);
+                        }
+#pragma unroll
+                        for (int o = 8; o; o >>= 1)
+#pragma unroll
+                            for (int i = 0; i < o; i++) {
+                                const bool up = lane & o;
+                                x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
+                            }
+                        x[0] = max_bf16x2(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
+                        if (lane < 16) {
+                            sm.part[warp][32 * hf + 2 * lane] = __uint_as_float(x[0] << 16);
+                            sm.part[warp][32 * hf + 2 * lane + 1] = __uint_as_float(x[0] & 0xffff0000u);
                         }
                     }
-#pragma unroll
-                    for (int o = 16; o; o >>= 1)
-#pragma unroll
-                        for (int i = 0; i < o; i++) {
-                            const bool up = lane & o;
-                            x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
-                        }
-                    sm.part[warp][2 * lane] = __uint_as_float(x[0] << 16);
-                    sm.part[warp][2 * lane + 1] = __uint_as_float(x[0] & 0xffff0000u);
                     soft_sync();
                     if (tid < AK_HEADS) {
                         const float old = sm.m[tid];
@@ -530,7 +556,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     }
                 }
                 uint32_t top = 0;                        // the largest numerator: as BF16 bits they compare like numbers
-#pragma unroll
+#pragma unroll 1
                 for (int hf = 0; hf < 2; hf++) {
                     uint32_t s[32];
                     tmem_ld32(tmem_s + lanes + 32 * hf, s);
@@ -580,6 +606,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
             if (lane < 8) sm.part[warp][8 * lane + i] = l[i];
         }
+        soft_sync();
+        if (tid < AK_HEADS) {
+            const float m = sm.m[tid], sum = (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]);
+            sm.ml[tid] = make_float2(m, sum);
+            // the only CTA of its row: what its part is multiplied by, while the last MMAs run
+            const float sk = sink * LOG2E, top = fmaxf(sk, m), den = ex2(sk - top) + sum * ex2(m - top);
+            sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(m - top) / den;
+        }
     }
     if (warp < AK_MMA) {
         if (!warp_wait(&sm.o_done, 0u, s_abort)) fail = 56;
@@ -590,39 +624,37 @@ attn_kv8_kernel(const AttnKv8Args a) {
 
     // channels per receiving CTA: whole warps of 32, and the parts of all CTAs fit the place of panels and queries
     const int slice = (a.d / C + 31) & ~31;
-    if (tid < AK_HEADS) sm.ml[tid] = make_float2(sm.m[tid], (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]));
     if (C > 1) {
         cluster_wait();                                  // every CTA of the cluster has started
         cluster_arrive();
         cluster_wait();                                  // all references and sums are there, all panels have been read
-    }
-    if (tid < AK_HEADS) {
-        const float sk2 = sm.sink[tid];
-        float2 ml[AK_MAX_C];
-#pragma unroll
-        for (int r = 0; r < AK_MAX_C; r++) {
-            ml[r] = make_float2(AK_NONE, 0.f);
-            if (r == 0 || r < C)
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                             : "=f"(ml[r].x), "=f"(ml[r].y) : "r"(cluster_addr(smem_u32(&sm.ml[tid]), r)));
+        float2 *ml = reinterpret_cast<float2 *>(smem + AK_P_OFF);        // [C][64], in the place of P
+        for (int i = tid; i < C * AK_HEADS; i += AK_THREADS) {
+            float2 v;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                         : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(smem_u32(&sm.ml[i & (AK_HEADS - 1)]), i / AK_HEADS)));
+            ml[i] = v;
         }
-        float top = fmaxf(sk2, AK_NONE);
-#pragma unroll
-        for (int r = 0; r < AK_MAX_C; r++) top = fmaxf(top, ml[r].x);
-        float den = ex2(sk2 - top);
-#pragma unroll
-        for (int r = 0; r < AK_MAX_C; r++)
-            if (r == 0 || r < C) den += ml[r].y * ex2(ml[r].x - top);
-        sm.f[tid] = sk2 == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[tid].x - top) / den;
+        __syncthreads();
+        if (tid < AK_HEADS) {
+            const float sk = sink * LOG2E;
+            float top = fmaxf(sk, AK_NONE), den = 0.f;
+#pragma unroll 4
+            for (int r = 0; r < C; r++) top = fmaxf(top, ml[r * AK_HEADS + tid].x);
+#pragma unroll 4
+            for (int r = 0; r < C; r++) den += ml[r * AK_HEADS + tid].y * ex2(ml[r * AK_HEADS + tid].x - top);
+            den += ex2(sk - top);
+            sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[tid].x - top) / den;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
+    const bool wide = C > 1 || !a.o_bf16;                // f32 in shared memory
     if (warp < 16) {
         const int quad = warp & 3, hh = (warp >> 2 & 1) * 32;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        float f[32];
-#pragma unroll
-        for (int k = 0; k < 32; k++) f[k] = sm.f[hh + k];
+        const float4 *f = reinterpret_cast<const float4 *>(sm.f + hh);
+#pragma unroll 1
         for (int i = warp >> 3; i < NPAIR; i += 2) {
             const int ch0 = i * 128 + quad * 32;
             if (ch0 >= a.d) break;
@@ -632,25 +664,23 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 tmem_ld32(tmem + lanes + i * AK_HEADS + hh, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             }
+            // A warp's 32 channels of one head are one piece: here [head][channel], the output's rows; or [CTA][head][channel] in
+            // the CTA that owns the channels
+            const int to = ch0 / slice;
+            const uint32_t base = C > 1 ? cluster_addr(smem_u32(smem), to) + (((uint32_t)rank * AK_HEADS + hh) * slice + (ch - to * slice)) * 4
+                                        : smem_u32(smem) + (hh * a.d + ch) * (wide ? 4 : 2);
+            const uint32_t step = (C > 1 ? slice : a.d) * (wide ? 4 : 2);
 #pragma unroll
-            for (int k = 0; k < 32; k++) v[k] = any ? __float_as_uint(__uint_as_float(v[k]) * f[k]) : 0u;
-            if (C > 1) {
-                // a warp's 32 channels of one head are one piece of 128 bytes (16 bytes of 32 rows took four times as long)
-                const int to = ch0 / slice;
-                const uint32_t base = cluster_addr(smem_u32(smem), to) + (((uint32_t)rank * AK_HEADS + hh) * slice + (ch - to * slice)) * 4;
+            for (int k = 0; k < 32; k += 4) {
+                const float4 g = f[k / 4];
+                const float x[4] = {__uint_as_float(v[k]) * g.x, __uint_as_float(v[k + 1]) * g.y, __uint_as_float(v[k + 2]) * g.z,
+                                    __uint_as_float(v[k + 3]) * g.w};
 #pragma unroll
-                for (int k = 0; k < 32; k++)
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(base + k * slice * 4), "r"(v[k]) : "memory");
-            } else if (a.o_bf16) {
-                const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * 2;
-#pragma unroll
-                for (int k = 0; k < 32; k++)
-                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + k * a.d * 2), "h"((uint16_t)bf16x2_rn(__uint_as_float(v[k]), 0.f)));
-            } else {
-                const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * 4;
-#pragma unroll
-                for (int k = 0; k < 32; k++)
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + k * a.d * 4), "r"(bf16x2_rn(__uint_as_float(v[k]), 0.f) << 16));
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t u = !any ? 0u : C > 1 ? __float_as_uint(x[j]) : bf16x2_rn(0.f, x[j]);
+                    if (wide) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(base + (k + j) * step), "r"(u) : "memory");
+                    else asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + (k + j) * step), "h"((uint16_t)(u >> 16)));
+                }
             }
         }
     }
@@ -661,12 +691,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
         if (!*s_abort) {
             const float *part = reinterpret_cast<const float *>(smem) + lane;
             const int n = min(slice, a.d - rank * slice) / 32;           // pieces of 32 channels
+#pragma unroll 1
             for (int u = warp; u < n * (AK_HEADS / 2); u += AK_MMA + 1) {
                 const int local = u % n * 32, hd = u / n * 2;
                 float v[2] = {0.f, 0.f};
+#pragma unroll 4
                 for (int r = 0; r < C; r++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) v[k] += part[(size_t)(r * AK_HEADS + hd + k) * slice + local];
+                    for (int k = 0; k < 2; k++) v[k] += part[(r * AK_HEADS + hd + k) * slice + local];
                 ak_put(a, o_at, rank * slice + local + lane, hd, nh, v);
             }
         }
@@ -676,12 +708,13 @@ attn_kv8_kernel(const AttnKv8Args a) {
         // the heads of this CTA are one piece of the output
         if (tid == 0 && !*s_abort) {
             const uint32_t bytes = (uint32_t)(nh * a.d) * (a.o_bf16 ? 2u : 4u);
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;"
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;"
                          ::"l"(static_cast<uint8_t *>(a.o) + o_at * (a.o_bf16 ? 2 : 4)), "r"(smem_u32(smem)), "r"(bytes) : "memory");
         }
     }
     if (fail) {
         atomicCAS(a.status, 0, fail);
+#pragma unroll 1
         for (int i = 0; i < 2000; i++) __nanosleep(1000);   // MMAs already issued end
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
