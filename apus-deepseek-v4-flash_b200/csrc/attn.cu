@@ -1044,11 +1044,8 @@ __global__ void compact_ids_kernel(const int32_t *__restrict__ idxs, int idxw,
 }
 
 // Scores / compacted ids between the kernels of a call: the caller's scratch (a model object keeps its own), else a
-// buffer of the library that belongs to the call's stream.  Calls on several streams never share one (a shared one
-// would let a call read the ids another is writing, or take the walk flags of another's rows); a call holds the lock
-// until its last launch, so that those of two threads on one stream do not mix and none loses its buffer to a growing
-// one.  A call that is being recorded gets memory that its graph owns.  At most SCR_MAX buffers are kept, the longest
-// unused one makes room for a new stream's, apus_cuda_disable frees them all.
+// buffer of the library that belongs to the call's stream (CallScratch, runtime.cuh).  At most SCR_MAX of them are kept, the
+// longest unused one makes room for a new stream's, apus_cuda_disable frees them all.
 #define SCR_MAX 16
 struct ScrSlot {
     int dev;
@@ -1068,44 +1065,35 @@ static void scr_release() {
 struct ScrReg { ScrReg() { on_disable(scr_release, nullptr); } };
 static ScrReg g_scr_reg;
 
-struct CallScratch {
-    std::unique_lock<std::mutex> lock;
-    cudaStream_t st;
-    void *p = nullptr;
-    bool recorded = false;
-    explicit CallScratch(cudaStream_t s) : st(s) {}
-    ~CallScratch() { if (recorded && p) cudaFreeAsync(p, st); }
-    CallScratch(const CallScratch &) = delete;
-    CallScratch &operator=(const CallScratch &) = delete;
-    int get(size_t bytes) {
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        APUS_CUDA_OK(cudaStreamIsCapturing(st, &cs));
-        if (cs != cudaStreamCaptureStatusNone) {
-            recorded = true;
-            APUS_CUDA_OK(cudaMallocAsync(&p, bytes, st));
-            return 0;
-        }
-        int dev = 0;
-        APUS_CUDA_OK(cudaGetDevice(&dev));
-        const std::thread::id th = st == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id();
-        lock = std::unique_lock<std::mutex>(g_scr_mu);
-        ScrSlot *slot = nullptr, *idle = nullptr;
-        for (ScrSlot &s : g_scr) {
-            if (s.dev == dev && s.st == st && s.th == th) slot = &s;
-            if (s.dev == dev && (!idle || s.used < idle->used)) idle = &s;
-        }
-        if (!slot && (g_scr.size() < SCR_MAX || !idle)) {
-            g_scr.push_back(ScrSlot{dev, st, th, DevBuf(), 0});
-            slot = &g_scr.back();
-        } else if (!slot) {
-            APUS_CUDA_OK(cudaDeviceSynchronize());         // another stream may still be using it
-            slot = idle;
-            slot->st = st; slot->th = th;
-        }
-        slot->used = ++g_scr_calls;
-        return slot->buf.get(bytes, &p);
+CallScratch::~CallScratch() { if (recorded && p) cudaFreeAsync(p, st); }
+int CallScratch::get(size_t bytes) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    APUS_CUDA_OK(cudaStreamIsCapturing(st, &cs));
+    if (cs != cudaStreamCaptureStatusNone) {
+        recorded = true;
+        APUS_CUDA_OK(cudaMallocAsync(&p, bytes, st));
+        return 0;
     }
-};
+    int dev = 0;
+    APUS_CUDA_OK(cudaGetDevice(&dev));
+    const std::thread::id th = st == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id();
+    lock = std::unique_lock<std::mutex>(g_scr_mu);
+    ScrSlot *slot = nullptr, *idle = nullptr;
+    for (ScrSlot &s : g_scr) {
+        if (s.dev == dev && s.st == st && s.th == th) slot = &s;
+        if (s.dev == dev && (!idle || s.used < idle->used)) idle = &s;
+    }
+    if (!slot && (g_scr.size() < SCR_MAX || !idle)) {
+        g_scr.push_back(ScrSlot{dev, st, th, DevBuf(), 0});
+        slot = &g_scr.back();
+    } else if (!slot) {
+        APUS_CUDA_OK(cudaDeviceSynchronize());         // another stream may still be using it
+        slot = idle;
+        slot->st = st; slot->th = th;
+    }
+    slot->used = ++g_scr_calls;
+    return slot->buf.get(bytes, &p);
+}
 // Layout of that scratch: scores, compacted ids, their counts, denominators, the walk flags of P.V.
 struct SaScratch {
     size_t ids, ns, den, bad, bytes;

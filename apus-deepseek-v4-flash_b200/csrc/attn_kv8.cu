@@ -26,6 +26,7 @@ struct AttnKv8Args {
     float scale;
     int q_bf16, o_bf16;
     int cluster, unit;           // CTAs per query row, tokens per tile (a multiple of 16 up to 112)
+    float *part;                 // [CTA]: O^T of a part as [64][d], then its 64 references and sums; where a row has several CTAs
     int *status;
 };
 
@@ -78,8 +79,9 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // precision; only then is the accumulator scaled.  Sums of numerators stay in each thread until the end.
 //
 // A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA
-// publishes its references and sums, scales its part of O^T and stores it into the shared memory of the CTA that owns the
-// channels, which adds the parts in rank order: one launch, no scratch, the same bits every time.
+// writes its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts
+// of its share of the heads in rank order: one launch, the same bits every time.  Through L2 and not through distributed
+// shared memory, which moves 15 bytes a cycle into an SM however it is asked (128 KB took 13,000 cycles; so 6,000).
 //
 // Warps 0 to 3: softmax.  Warps 4 to 17: rows, fetched into registers a tile ahead and dequantised into shared memory, the
 // first seven of them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one
@@ -91,22 +93,24 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 constexpr int AK_TILE = 112, AK_HEADS = 64;
 constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
+static_assert(8 * 32 * AK_MMA >= AK_HEADS * KV8_MAX_D / 8, "eight pieces of a thread are all queries");
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
+constexpr int AK_MOST_PARTS = 1024;                     // 135 MB of scratch
 constexpr uint32_t AK_SLACK = 64;
 constexpr float AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 
 struct AkMisc {
-    float2 ml[AK_HEADS];                                // reference and sum of this CTA
     alignas(16) float m[AK_HEADS];
     alignas(16) float f[AK_HEADS];
-    float part[4][AK_HEADS];
+    alignas(16) float part[4][AK_HEADS];
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
 };
 constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc);
 static_assert(AK_SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
-static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32, or the parts of all CTAs, in the place of panels and queries");
+static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32 in the place of panels and queries");
+static_assert(sizeof(((AkMisc *)0)->part) >= 64 * sizeof(float2), "references and sums of a share of the heads");
 
 // barriers of the softmax warps
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -118,11 +122,6 @@ __device__ __forceinline__ bool soft_any(bool p) {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 // A wait of a whole warp, which goes on together; false when it ran out or another one did.  One loop, not unrolled, like the
 // others below: this kernel's roles run through their code once per tile, and what the instruction caches do not hold they
 // wait for (124 KB of code, half of it unrolled waits, took 20 % longer than 60 KB).
@@ -295,19 +294,62 @@ struct TileRows {
     }
 };
 
-// Two heads of o[head][ch]: lane = channel
-__device__ __forceinline__ void ak_put(const AttnKv8Args &a, size_t at, int ch, int hd, int nh, const float (&v)[2]) {
-    if (!a.o_bf16) {
-        float *o = static_cast<float *>(a.o) + at + (size_t)hd * a.d + ch;
-        if (hd < nh) o[0] = __uint_as_float(bf16x2_rn(v[0], 0.f) << 16);
-        if (hd + 1 < nh) o[a.d] = __uint_as_float(bf16x2_rn(v[1], 0.f) << 16);
-        return;
+// The parts of a row's C CTAs, joined for this CTA's share of the heads: 4 channels of a head at a time, sixteen loads in flight
+template <int C>
+__device__ __noinline__ void ak_join(float2 *ml, const float *parts, int d, const float *sink, void *o, int o_bf16, int rank, int nh) {
+    const int per = (nh + C - 1) / C, lo = rank * per, n = min(per, nh - lo), tid = threadIdx.x;
+    const size_t part_size = AK_HEADS * d + 2 * AK_HEADS;
+    // ml [head][CTA]: reference and sum, then what the part is multiplied by
+    for (int i = tid; i < n * C; i += AK_THREADS)
+        ml[i] = __ldcg(reinterpret_cast<const float2 *>(parts + (i % C) * part_size + AK_HEADS * d) + lo + i / C);
+    __syncthreads();
+    if (tid < n) {
+        const float sk = sink ? sink[lo + tid] * LOG2E : -INFINITY;
+        float top = fmaxf(sk, AK_NONE), den = 0.f;
+#pragma unroll
+        for (int r = 0; r < C; r++) top = fmaxf(top, ml[tid * C + r].x);
+#pragma unroll
+        for (int r = 0; r < C; r++) den += ml[tid * C + r].y * ex2(ml[tid * C + r].x - top);
+        den += ex2(sk - top);
+#pragma unroll
+        for (int r = 0; r < C; r++) {
+            const float2 v = ml[tid * C + r];
+            // a part without tokens has not been written
+            ml[tid * C + r].x = v.x == AK_NONE && v.y == 0.f || sk == INFINITY || den == 0.f ? -1.f : ex2(v.x - top) / den;
+        }
     }
-    // neighbours trade, so that each stores two channels of one head
-    const bool odd = ch & 1;
-    const float other = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1);
-    const uint32_t w = odd ? bf16x2_rn(other, v[1]) : bf16x2_rn(v[0], other);
-    if (hd + odd < nh) *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.o) + at + (size_t)(hd + odd) * a.d + (ch & ~1)) = w;
+    __syncthreads();
+    constexpr int U = 16 / C;
+    const int per_head = d / 4, total = n * per_head;
+#pragma unroll 1
+    for (int u0 = tid; u0 < total; u0 += U * AK_THREADS) {
+        float4 x[U][C];
+        float w[U][C];
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const int u = u0 + k * AK_THREADS, hd = u / per_head, c = u - hd * per_head;
+#pragma unroll
+            for (int r = 0; r < C; r++) {
+                w[k][r] = u < total ? ml[hd * C + r].x : -1.f;
+                x[k][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (w[k][r] >= 0.f || w[k][r] != w[k][r]) x[k][r] = __ldcg(reinterpret_cast<const float4 *>(parts + r * part_size + (lo + hd) * d) + c);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const int u = u0 + k * AK_THREADS;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int r = 0; r < C; r++) {
+                s.x += w[k][r] * x[k][r].x; s.y += w[k][r] * x[k][r].y; s.z += w[k][r] * x[k][r].z; s.w += w[k][r] * x[k][r].w;
+            }
+            if (u >= total) break;
+            const uint32_t p = bf16x2_rn(s.x, s.y), q = bf16x2_rn(s.z, s.w);
+            const size_t i = (size_t)lo * d + (size_t)u * 4;
+            if (o_bf16) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + i) = make_uint2(p, q);
+            else *reinterpret_cast<uint4 *>(static_cast<uint32_t *>(o) + i) = make_uint4(p << 16, p & 0xffff0000u, q << 16, q & 0xffff0000u);
+        }
+    }
 }
 
 template <bool TAIL>
@@ -322,22 +364,24 @@ attn_kv8_kernel(const AttnKv8Args a) {
     const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * AK_HEADS, nh = min(AK_HEADS, a.h - h0);
     const uint32_t row = blockIdx.x / (unsigned)C, seq = row / (uint32_t)a.rows_per_seq;
     const Kv8Seq at(a, seq);
+    const size_t part_size = AK_HEADS * a.d + 2 * AK_HEADS;
+    float *part = a.part + (blockIdx.y * (size_t)gridDim.x + blockIdx.x) * part_size;
     const int32_t *ids = a.idxs + (size_t)row * a.idxw;
     const int n_tiles = (a.idxw + a.unit - 1) / a.unit, NP = a.d / 64, NPAIR = (NP + 1) / 2;
 
     // What the first tile waits for is asked for before anything else: its ids, sinks, and the queries, 8 channels at a time,
-    // four times at once, by all warps but the one of the MMAs
+    // eight times at once (which is all of them), by all warps but the one of the MMAs
     TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
     int tile = rank;
     cur.load(a, ids, tile, lane);
-    uint4 qv[4][2];
+    uint4 qv[8][2];
     const int per_head = a.d / 8, q_heads = 32 * AK_MMA / per_head, q_rest = 32 * AK_MMA % per_head;
     int q_head = tid / per_head, q_c = tid % per_head;   // of this thread's next piece
     auto ask = [&]() {
         const uint8_t *q = static_cast<const uint8_t *>(a.q) + ((size_t)row * a.h + h0) * a.d * (a.q_bf16 ? 2 : 4);
         int hd = q_head, c = q_c;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 8; k++) {
             const uint8_t *p = q + (uint32_t)(hd < nh ? hd * per_head + c : 0) * (a.q_bf16 ? 16u : 32u);
             qv[k][0] = ldg16_if(p, hd < nh);
             qv[k][1] = ldg16_if(p + 16, hd < nh && !a.q_bf16);
@@ -348,7 +392,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     };
     auto place = [&]() {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 8; k++) {
             uint4 v = qv[k][0];
             if (!a.q_bf16)
                 v = make_uint4(bf16x2_rn(__uint_as_float(v.x), __uint_as_float(v.y)), bf16x2_rn(__uint_as_float(v.z), __uint_as_float(v.w)),
@@ -384,7 +428,6 @@ attn_kv8_kernel(const AttnKv8Args a) {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (C > 1) cluster_arrive();                        // this CTA has started: its shared memory may be stored to
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0), tmem_s = tmem + 4 * AK_HEADS;
 
     // A wait that runs out sets the abort flag, after which every other wait gives up soon; all loops and barriers are gone
@@ -403,13 +446,11 @@ attn_kv8_kernel(const AttnKv8Args a) {
     settle();
     const bool any = more;                               // there is an output to read
 
-    if (warp != AK_MMA) place();
-    auto queries = [&]() {                               // the rest of them
-#pragma unroll 1
-        while (__any_sync(0xffffffffu, q_head < AK_HEADS)) { ask(); place(); }
+    if (warp != AK_MMA) {
+        place();
         proxy_fence();
         mbar_arrive_warp(&sm.q_full, lane);
-    };
+    }
     if (warp == AK_MMA) {
         const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
         const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
@@ -459,7 +500,6 @@ attn_kv8_kernel(const AttnKv8Args a) {
         const int x0 = ((2 * sub) ^ (r0 & 7)) * 16, x1 = ((2 * sub + 1) ^ (r0 & 7)) * 16;
         TileRows<TAIL> rows;
         if (n && more) rows.load(at, cur, w, lane, from, scales, n_codes, n);
-        queries();
         while (n && more) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
@@ -484,7 +524,6 @@ attn_kv8_kernel(const AttnKv8Args a) {
         const int token = tid;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const float cs = a.scale * LOG2E;
-        queries();
         // sums of numerators: of 8 heads, over the 8 tokens in a row that this thread adds up of every tile
         const int lh = tid & 7, lt = (tid >> 3) * 8;
         float l[8];
@@ -609,7 +648,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         soft_sync();
         if (tid < AK_HEADS) {
             const float m = sm.m[tid], sum = (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]);
-            sm.ml[tid] = make_float2(m, sum);
+            if (C > 1) reinterpret_cast<float2 *>(part + AK_HEADS * a.d)[tid] = make_float2(m, sum);
             // the only CTA of its row: what its part is multiplied by, while the last MMAs run
             const float sk = sink * LOG2E, top = fmaxf(sk, m), den = ex2(sk - top) + sum * ex2(m - top);
             sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(m - top) / den;
@@ -622,35 +661,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     __syncthreads();
 
-    // channels per receiving CTA: whole warps of 32, and the parts of all CTAs fit the place of panels and queries
-    const int slice = (a.d / C + 31) & ~31;
-    if (C > 1) {
-        cluster_wait();                                  // every CTA of the cluster has started
-        cluster_arrive();
-        cluster_wait();                                  // all references and sums are there, all panels have been read
-        float2 *ml = reinterpret_cast<float2 *>(smem + AK_P_OFF);        // [C][64], in the place of P
-        for (int i = tid; i < C * AK_HEADS; i += AK_THREADS) {
-            float2 v;
-            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-                         : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(smem_u32(&sm.ml[i & (AK_HEADS - 1)]), i / AK_HEADS)));
-            ml[i] = v;
-        }
-        __syncthreads();
-        if (tid < AK_HEADS) {
-            const float sk = sink * LOG2E;
-            float top = fmaxf(sk, AK_NONE), den = 0.f;
-#pragma unroll 4
-            for (int r = 0; r < C; r++) top = fmaxf(top, ml[r * AK_HEADS + tid].x);
-#pragma unroll 4
-            for (int r = 0; r < C; r++) den += ml[r * AK_HEADS + tid].y * ex2(ml[r * AK_HEADS + tid].x - top);
-            den += ex2(sk - top);
-            sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(sm.ml[tid].x - top) / den;
-        }
-        __syncthreads();
-    }
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
-    const bool wide = C > 1 || !a.o_bf16;                // f32 in shared memory
-    if (warp < 16) {
+    if (warp < 16 && (any || C == 1)) {
         const int quad = warp & 3, hh = (warp >> 2 & 1) * 32;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const float4 *f = reinterpret_cast<const float4 *>(sm.f + hh);
@@ -664,12 +676,15 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 tmem_ld32(tmem + lanes + i * AK_HEADS + hh, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             }
-            // A warp's 32 channels of one head are one piece: here [head][channel], the output's rows; or [CTA][head][channel] in
-            // the CTA that owns the channels
-            const int to = ch0 / slice;
-            const uint32_t base = C > 1 ? cluster_addr(smem_u32(smem), to) + (((uint32_t)rank * AK_HEADS + hh) * slice + (ch - to * slice)) * 4
-                                        : smem_u32(smem) + (hh * a.d + ch) * (wide ? 4 : 2);
-            const uint32_t step = (C > 1 ? slice : a.d) * (wide ? 4 : 2);
+            if (C > 1) {
+                float *p = part + hh * a.d + ch;
+#pragma unroll
+                for (int k = 0; k < 32; k++, p += a.d)
+                    if (hh + k < nh) __stcg(p, __uint_as_float(v[k]));
+                continue;
+            }
+            // the output's rows in shared memory, a warp's 32 channels of a head at a time
+            const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * (a.o_bf16 ? 2 : 4), step = a.d * (a.o_bf16 ? 2 : 4);
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
                 const float4 g = f[k / 4];
@@ -677,9 +692,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
                                     __uint_as_float(v[k + 3]) * g.w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t u = !any ? 0u : C > 1 ? __float_as_uint(x[j]) : bf16x2_rn(0.f, x[j]);
-                    if (wide) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(base + (k + j) * step), "r"(u) : "memory");
-                    else asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + (k + j) * step), "h"((uint16_t)(u >> 16)));
+                    const uint32_t u = any ? bf16x2_rn(0.f, x[j]) : 0u;
+                    if (a.o_bf16) asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + (k + j) * step), "h"((uint16_t)(u >> 16)));
+                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + (k + j) * step), "r"(u));
                 }
             }
         }
@@ -687,20 +702,15 @@ attn_kv8_kernel(const AttnKv8Args a) {
     if (C > 1) {
         __syncwarp();
         cluster_arrive();
-        cluster_wait();                                  // the parts of this CTA's channels are in; nothing remote after this
+        cluster_wait();                                  // the parts of all CTAs are written
         if (!*s_abort) {
-            const float *part = reinterpret_cast<const float *>(smem) + lane;
-            const int n = min(slice, a.d - rank * slice) / 32;           // pieces of 32 channels
-#pragma unroll 1
-            for (int u = warp; u < n * (AK_HEADS / 2); u += AK_MMA + 1) {
-                const int local = u % n * 32, hd = u / n * 2;
-                float v[2] = {0.f, 0.f};
-#pragma unroll 4
-                for (int r = 0; r < C; r++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) v[k] += part[(r * AK_HEADS + hd + k) * slice + local];
-                ak_put(a, o_at, rank * slice + local + lane, hd, nh, v);
-            }
+            const float *parts = part - (size_t)rank * part_size, *sinks = a.sink ? a.sink + h0 : nullptr;
+            float2 *ml = reinterpret_cast<float2 *>(sm.part);
+            void *o = static_cast<uint8_t *>(a.o) + o_at * (a.o_bf16 ? 2 : 4);
+            if (C == 2) ak_join<2>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            else if (C == 4) ak_join<4>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            else if (C == 8) ak_join<8>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            else ak_join<16>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
         }
     } else {
         proxy_fence();
@@ -730,7 +740,7 @@ void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluste
     *unit = 16;
     for (int i = 0; i < 5; i++) {
         const int C = 1 << i;
-        if (slots[i] < 1) continue;
+        if (slots[i] < 1 || (i && rows << i > AK_MOST_PARTS)) continue;
         const int k = idxw > AK_TILE * C ? (idxw + AK_TILE * C - 1) / (AK_TILE * C) : 1;      // tiles of the CTA with the most
         const int u = idxw ? ((idxw + C * k - 1) / (C * k) + 15) & ~15 : 16;
         const double waves = (double)((rows + slots[i] - 1) / slots[i]);
@@ -777,6 +787,9 @@ int attn_kv8(AttnKv8Args a, cudaStream_t st) {
     if (!dev || !a.status) return 1;
     const unsigned hb = (unsigned)ceil_div(a.h, AK_HEADS);
     attn_kv8_shape(a.idxw, (long long)a.rows * hb, dev->slots[a.rd != 0], &a.cluster, &a.unit);
+    CallScratch scratch(st);
+    if (a.cluster > 1 && scratch.get((size_t)a.rows * hb * a.cluster * (AK_HEADS * a.d + 2 * AK_HEADS) * sizeof(float))) return 1;
+    a.part = static_cast<float *>(scratch.p);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cudaLaunchAttribute at[2];
@@ -816,6 +829,6 @@ extern "C" int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const fl
     APUS_REQUIRE(aligned16(q) && aligned16(o), "sparse_attn_kv8: queries and output must start on a 16-byte boundary");
     if (ensure_enabled()) return 1;
     const AttnKv8Args a = {q, sink, idxs, kv_a, kv_b, o, na, nb, kv_a_stride, kv_b_stride, h, d, rd, idxw, rows, rows_per_seq,
-                           scale, q_bf16 != 0, o_bf16 != 0, 1, 16, nullptr};
+                           scale, q_bf16 != 0, o_bf16 != 0, 1, 16, nullptr, nullptr};
     return attn_kv8(a, (cudaStream_t)stream);
 }

@@ -25,6 +25,22 @@ struct DevBuf {
     template <class T> T *as() const { return static_cast<T *>(p); }
 };
 
+// Scratch of one call that belongs to the call's stream.  Calls on several streams never share one (a shared one would
+// let a call read what another is writing); a call holds the lock until its last launch, so that those of two threads
+// on one stream do not mix and none loses its buffer to a growing one.  A call that is being recorded gets memory that its
+// graph owns.
+struct CallScratch {
+    std::unique_lock<std::mutex> lock;
+    cudaStream_t st;
+    void *p = nullptr;
+    bool recorded = false;
+    explicit CallScratch(cudaStream_t s) : st(s) {}
+    ~CallScratch();                                // attn.cu
+    CallScratch(const CallScratch &) = delete;
+    CallScratch &operator=(const CallScratch &) = delete;
+    int get(size_t bytes);
+};
+
 // One quantised matrix resident in HBM in the fragment-tiled layout.
 struct DevQW {
     int fmt = 0;              // 4 or 8
