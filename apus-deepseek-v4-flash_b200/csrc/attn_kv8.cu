@@ -46,6 +46,11 @@ struct Kv8Seq {
         return reinterpret_cast<const uint8_t *>((id < na ? a : b) + (uintptr_t)(uint32_t)id * bytes);
     }
 };
+__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 // 16 or 4 bytes of global memory, or zeros; here and not where the value is first used, and without a branch
 __device__ __forceinline__ uint4 ldg16_if(const uint8_t *p, bool yes) {
     uint4 v;
@@ -75,7 +80,7 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // stores them as one contiguous piece of a row of P.
 //
 // The softmax is one pass with a reference per head instead of the running maximum: it is set to the first tile's maximum
-// and stays until a score exceeds it by more than 2^AK_SLACK, which in f32 and BF16, floating as both are, costs no
+// and stays until a score exceeds it by more than AK_SLACK powers of two, which in f32 and BF16, floating as both are, costs no
 // precision; only then is the accumulator scaled.  Sums of numerators stay in each thread until the end.
 //
 // A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA
@@ -110,7 +115,6 @@ struct AkMisc {
 constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc);
 static_assert(AK_SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
 static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32 in the place of panels and queries");
-static_assert(sizeof(((AkMisc *)0)->part) >= 64 * sizeof(float2), "references and sums of a share of the heads");
 
 // barriers of the softmax warps
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -294,60 +298,67 @@ struct TileRows {
     }
 };
 
-// The parts of a row's C CTAs, joined for this CTA's share of the heads: 4 channels of a head at a time, sixteen loads in flight
-template <int C>
-__device__ __noinline__ void ak_join(float2 *ml, const float *parts, int d, const float *sink, void *o, int o_bf16, int rank, int nh) {
+// The parts of a row's C CTAs, joined for this CTA's share of the heads: U times 4 channels of a head and R of the parts at a
+// time, eight loads in flight
+template <int U, int R>
+__device__ __forceinline__ void ak_join(int C, float *w, const float *parts, int d, const float *sink, void *o, int o_bf16, int rank, int nh) {
     const int per = (nh + C - 1) / C, lo = rank * per, n = min(per, nh - lo), tid = threadIdx.x;
-    const size_t part_size = AK_HEADS * d + 2 * AK_HEADS;
-    // ml [head][CTA]: reference and sum, then what the part is multiplied by
-    for (int i = tid; i < n * C; i += AK_THREADS)
-        ml[i] = __ldcg(reinterpret_cast<const float2 *>(parts + (i % C) * part_size + AK_HEADS * d) + lo + i / C);
-    __syncthreads();
-    if (tid < n) {
-        const float sk = sink ? sink[lo + tid] * LOG2E : -INFINITY;
-        float top = fmaxf(sk, AK_NONE), den = 0.f;
-#pragma unroll
-        for (int r = 0; r < C; r++) top = fmaxf(top, ml[tid * C + r].x);
-#pragma unroll
-        for (int r = 0; r < C; r++) den += ml[tid * C + r].y * ex2(ml[tid * C + r].x - top);
-        den += ex2(sk - top);
-#pragma unroll
-        for (int r = 0; r < C; r++) {
-            const float2 v = ml[tid * C + r];
-            // a part without tokens has not been written
-            ml[tid * C + r].x = v.x == AK_NONE && v.y == 0.f || sk == INFINITY || den == 0.f ? -1.f : ex2(v.x - top) / den;
+    const uint32_t part_size = AK_HEADS * d + 2 * AK_HEADS;
+    if (tid < AK_HEADS) {
+        // lane i of a head's C lanes: reference and sum of part i; w [head][part]: what a part is multiplied by, -1 for one
+        // without tokens, which has not been written
+        const int hd = tid / C, r = tid % C;
+        float2 v = make_float2(AK_NONE, 0.f);
+        float sk = -INFINITY;
+        if (hd < n) {
+            v = __ldcg(reinterpret_cast<const float2 *>(parts + r * part_size + AK_HEADS * d) + lo + hd);
+            if (sink) sk = sink[lo + hd] * LOG2E;
         }
+        float top = fmaxf(v.x, sk);
+        for (int m = 1; m < C; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+        float den = v.y * ex2(v.x - top);
+        for (int m = 1; m < C; m <<= 1) den += __shfl_xor_sync(0xffffffffu, den, m);
+        den += ex2(sk - top);
+        w[tid] = v.x == AK_NONE && v.y == 0.f || sk == INFINITY || den == 0.f ? -1.f : ex2(v.x - top) / den;
     }
     __syncthreads();
-    constexpr int U = 16 / C;
     const int per_head = d / 4, total = n * per_head;
 #pragma unroll 1
     for (int u0 = tid; u0 < total; u0 += U * AK_THREADS) {
-        float4 x[U][C];
-        float w[U][C];
+        float s[U][4];
+        const uint8_t *p[U];
+        const float *f[U];
 #pragma unroll
         for (int k = 0; k < U; k++) {
-            const int u = u0 + k * AK_THREADS, hd = u / per_head, c = u - hd * per_head;
+            const int u = min(u0 + k * AK_THREADS, total - 1);
+            s[k][0] = s[k][1] = s[k][2] = s[k][3] = 0.f;
+            p[k] = reinterpret_cast<const uint8_t *>(parts + lo * d + u * 4);
+            f[k] = w + u / per_head * C;
+        }
+#pragma unroll 1
+        for (int r0 = 0; r0 < C; r0 += R) {
+            uint4 x[U][R];
 #pragma unroll
-            for (int r = 0; r < C; r++) {
-                w[k][r] = u < total ? ml[hd * C + r].x : -1.f;
-                x[k][r] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (w[k][r] >= 0.f || w[k][r] != w[k][r]) x[k][r] = __ldcg(reinterpret_cast<const float4 *>(parts + r * part_size + (lo + hd) * d) + c);
-            }
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int r = 0; r < R; r++) x[k][r] = ldg16_if(p[k] + (r0 + r) * (part_size * 4), !(f[k][r0 + r] < 0.f));
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float g = f[k][r0 + r];
+                    s[k][0] += g * __uint_as_float(x[k][r].x); s[k][1] += g * __uint_as_float(x[k][r].y);
+                    s[k][2] += g * __uint_as_float(x[k][r].z); s[k][3] += g * __uint_as_float(x[k][r].w);
+                }
         }
 #pragma unroll
         for (int k = 0; k < U; k++) {
             const int u = u0 + k * AK_THREADS;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int r = 0; r < C; r++) {
-                s.x += w[k][r] * x[k][r].x; s.y += w[k][r] * x[k][r].y; s.z += w[k][r] * x[k][r].z; s.w += w[k][r] * x[k][r].w;
-            }
             if (u >= total) break;
-            const uint32_t p = bf16x2_rn(s.x, s.y), q = bf16x2_rn(s.z, s.w);
+            const uint32_t x = bf16x2_rn(s[k][0], s[k][1]), y = bf16x2_rn(s[k][2], s[k][3]);
             const size_t i = (size_t)lo * d + (size_t)u * 4;
-            if (o_bf16) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + i) = make_uint2(p, q);
-            else *reinterpret_cast<uint4 *>(static_cast<uint32_t *>(o) + i) = make_uint4(p << 16, p & 0xffff0000u, q << 16, q & 0xffff0000u);
+            if (o_bf16) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(o) + i) = make_uint2(x, y);
+            else *reinterpret_cast<uint4 *>(static_cast<uint32_t *>(o) + i) = make_uint4(x << 16, x & 0xffff0000u, y << 16, y & 0xffff0000u);
         }
     }
 }
@@ -355,7 +366,6 @@ __device__ __noinline__ void ak_join(float2 *ml, const float *parts, int d, cons
 template <bool TAIL>
 __global__ void __launch_bounds__(AK_THREADS, 1)
 attn_kv8_kernel(const AttnKv8Args a) {
-    APUS_PDL_WAIT();
     APUS_PDL_GO();
     extern __shared__ __align__(1024) uint8_t smem[];
     AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + AK_MISC_OFF);
@@ -369,8 +379,23 @@ attn_kv8_kernel(const AttnKv8Args a) {
     const int32_t *ids = a.idxs + (size_t)row * a.idxw;
     const int n_tiles = (a.idxw + a.unit - 1) / a.unit, NP = a.d / 64, NPAIR = (NP + 1) / 2;
 
-    // What the first tile waits for is asked for before anything else: its ids, sinks, and the queries, 8 channels at a time,
-    // eight times at once (which is all of them), by all warps but the one of the MMAs
+    // The barriers while the kernel before this one may still run, global memory only after it.  Tensor memory too: that
+    // kernel's CTAs may have yet to take theirs.
+    if (tid == 0) {
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) { mbar_init(&sm.full[i], AK_ROWS); mbar_init(&sm.empty[i], 1); }
+        mbar_init(&sm.q_full, AK_MMA);
+        mbar_init(&sm.s_full, 1);
+        mbar_init(&sm.p_ready, AK_SOFT);
+        mbar_init(&sm.o_done, 1);
+        *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
+    APUS_PDL_WAIT();
+
+    // What the first tile waits for: its ids, sinks, and the queries, 8 channels at a time, all at once, by all warps but the one
+    // of the MMAs.  In the place of heads that there are not a CTA has the first one's queries.
     TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
     int tile = rank;
     cur.load(a, ids, tile, lane);
@@ -382,9 +407,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
         int hd = q_head, c = q_c;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const uint8_t *p = q + (uint32_t)(hd < nh ? hd * per_head + c : 0) * (a.q_bf16 ? 16u : 32u);
-            qv[k][0] = ldg16_if(p, hd < nh);
-            qv[k][1] = ldg16_if(p + 16, hd < nh && !a.q_bf16);
+            const uint8_t *p = q + (uint32_t)((hd < nh ? hd * per_head : 0) + c) * (a.q_bf16 ? 16u : 32u);
+            qv[k][0] = ldg16(p);
+            if (!a.q_bf16) qv[k][1] = ldg16(p + 16);
             hd += q_heads;
             c += q_rest;
             if (c >= per_head) { c -= per_head; hd++; }
@@ -410,16 +435,6 @@ attn_kv8_kernel(const AttnKv8Args a) {
     if (warp != AK_MMA) ask();
     const float sink = a.sink && tid < nh ? a.sink[h0 + tid] : -INFINITY;        // of head tid
 
-    if (tid == 0) {
-        for (int i = 0; i < 4; i++) { mbar_init(&sm.full[i], AK_ROWS); mbar_init(&sm.empty[i], 1); }
-        mbar_init(&sm.q_full, AK_MMA);
-        mbar_init(&sm.s_full, 1);
-        mbar_init(&sm.p_ready, AK_SOFT);
-        mbar_init(&sm.o_done, 1);
-        *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
     if (warp == AK_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
@@ -705,12 +720,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
         cluster_wait();                                  // the parts of all CTAs are written
         if (!*s_abort) {
             const float *parts = part - (size_t)rank * part_size, *sinks = a.sink ? a.sink + h0 : nullptr;
-            float2 *ml = reinterpret_cast<float2 *>(sm.part);
             void *o = static_cast<uint8_t *>(a.o) + o_at * (a.o_bf16 ? 2 : 4);
-            if (C == 2) ak_join<2>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
-            else if (C == 4) ak_join<4>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
-            else if (C == 8) ak_join<8>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
-            else ak_join<16>(ml, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            if (C <= 4) ak_join<4, 2>(C, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            else ak_join<1, 8>(C, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
         }
     } else {
         proxy_fence();
