@@ -96,9 +96,9 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
 // comes of them is masked.)
 constexpr int AK_TILE = 112, AK_HEADS = 64;
-constexpr int AK_SOFT = 4, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
+constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
-static_assert(8 * 32 * AK_MMA >= AK_HEADS * KV8_MAX_D / 8, "eight pieces of a thread are all queries");
+constexpr int AK_ASK = (AK_HEADS * KV8_MAX_D / 8 + 32 * AK_MMA - 1) / (32 * AK_MMA);             // pieces of 8 query channels per thread
 constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
 constexpr int AK_MOST_PARTS = 1024;                     // 135 MB of scratch
 constexpr uint32_t AK_SLACK = 64;
@@ -107,7 +107,7 @@ constexpr float AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 struct AkMisc {
     alignas(16) float m[AK_HEADS];
     alignas(16) float f[AK_HEADS];
-    alignas(16) float part[4][AK_HEADS];
+    alignas(16) float part[AK_SOFT][AK_HEADS];
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
     int abort;
@@ -117,10 +117,10 @@ static_assert(AK_SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
 static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32 in the place of panels and queries");
 
 // barriers of the softmax warps
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool soft_any(bool p) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(r) : "r"((uint32_t)p) : "memory");
     return r != 0;
 }
@@ -399,14 +399,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
     TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
     int tile = rank;
     cur.load(a, ids, tile, lane);
-    uint4 qv[8][2];
+    uint4 qv[AK_ASK][2];
     const int per_head = a.d / 8, q_heads = 32 * AK_MMA / per_head, q_rest = 32 * AK_MMA % per_head;
     int q_head = tid / per_head, q_c = tid % per_head;   // of this thread's next piece
     auto ask = [&]() {
         const uint8_t *q = static_cast<const uint8_t *>(a.q) + ((size_t)row * a.h + h0) * a.d * (a.q_bf16 ? 2 : 4);
         int hd = q_head, c = q_c;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < AK_ASK; k++) {
             const uint8_t *p = q + (uint32_t)((hd < nh ? hd * per_head : 0) + c) * (a.q_bf16 ? 16u : 32u);
             qv[k][0] = ldg16(p);
             if (!a.q_bf16) qv[k][1] = ldg16(p + 16);
@@ -417,7 +417,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     };
     auto place = [&]() {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < AK_ASK; k++) {
             uint4 v = qv[k][0];
             if (!a.q_bf16)
                 v = make_uint4(bf16x2_rn(__uint_as_float(v.x), __uint_as_float(v.y)), bf16x2_rn(__uint_as_float(v.z), __uint_as_float(v.w)),
@@ -536,50 +536,47 @@ attn_kv8_kernel(const AttnKv8Args a) {
             done++;
         }
     } else {
-        const int token = tid;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        // a thread has one token and 32 of the heads
+        const int quad = warp & 3, hh = (warp >> 2) * 32, token = tid & 127;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const float cs = a.scale * LOG2E;
-        // sums of numerators: of 8 heads, over the 8 tokens in a row that this thread adds up of every tile
-        const int lh = tid & 7, lt = (tid >> 3) * 8;
+        // sums of numerators: of 8 heads, over the 4 tokens in a row that this thread adds up of every tile
+        const int lh = tid & 7, lt = (tid >> 3) * 4;
         float l[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) l[i] = 0.f;
         uint8_t *prow = smem + AK_P_OFF + token * 128;
-        const float4 *mp = reinterpret_cast<const float4 *>(sm.m);
+        const float4 *mp = reinterpret_cast<const float4 *>(sm.m + hh);
         while (more) {
-            const bool valid = (warp == 0 ? cur.id[0] : warp == 1 ? cur.id[1] : warp == 2 ? cur.id[2] : cur.id[3]) >= 0;
+            const bool valid = (quad == 0 ? cur.id[0] : quad == 1 ? cur.id[1] : quad == 2 ? cur.id[2] : cur.id[3]) >= 0;
             const uint32_t mask = valid ? ~0u : 0u;      // not a choice: the compiler would branch around every numerator
             tile += C;
             cur.load(a, ids, tile, lane);
             if (!warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (bool set = done == 0;; set = true) {
+                uint32_t s[32];
+                tmem_ld32(tmem_s + lanes + hh, s);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (set) {
                     // New references: the maxima over the tokens so far, as BF16 (they need not be exact), two heads in a register
-                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1 of a half.
-#pragma unroll 1
-                    for (int hf = 0; hf < 2; hf++) {
-                        uint32_t s[32], x[16];
-                        tmem_ld32(tmem_s + lanes + 32 * hf, s);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1 of this warp's.
+                    uint32_t x[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const uint32_t u = bf16x2_rn(__uint_as_float(s[2 * i]) * cs, __uint_as_float(s[2 * i + 1]) * cs);
-                            x[i] = (u & mask) | (0xff80ff80u & ~mask);
-                        }
-#pragma unroll
-                        for (int o = 8; o; o >>= 1)
-#pragma unroll
-                            for (int i = 0; i < o; i++) {
-                                const bool up = lane & o;
-                                x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
-                            }
-                        x[0] = max_bf16x2(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
-                        if (lane < 16) {
-                            sm.part[warp][32 * hf + 2 * lane] = __uint_as_float(x[0] << 16);
-                            sm.part[warp][32 * hf + 2 * lane + 1] = __uint_as_float(x[0] & 0xffff0000u);
-                        }
+                    for (int i = 0; i < 16; i++) {
+                        const uint32_t u = bf16x2_rn(__uint_as_float(s[2 * i]) * cs, __uint_as_float(s[2 * i + 1]) * cs);
+                        x[i] = (u & mask) | (0xff80ff80u & ~mask);
                     }
+#pragma unroll
+                    for (int o = 8; o; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < o; i++) {
+                            const bool up = lane & o;
+                            x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
+                        }
+                    x[0] = max_bf16x2(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
+                    if (lane < 16)
+                        *reinterpret_cast<float2 *>(&sm.part[quad][hh + 2 * lane]) = make_float2(__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u));
                     soft_sync();
                     if (tid < AK_HEADS) {
                         const float old = sm.m[tid];
@@ -589,50 +586,46 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     }
                     soft_sync();
                     if (done) {
+                        const float4 *f = reinterpret_cast<const float4 *>(sm.f + hh);
 #pragma unroll
                         for (int i = 0; i < 8; i++) l[i] *= sm.f[8 * lh + i];
 #pragma unroll 1
-                        for (int hf = 0; hf < 2; hf++) {
-                            float f[32];
+                        for (int i = 0; i < NPAIR; i++) {
+                            const uint32_t o = tmem + lanes + i * AK_HEADS + hh;
+                            tmem_ld32(o, s);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int k = 0; k < 32; k++) f[k] = sm.f[32 * hf + k];
-#pragma unroll 1
-                            for (int i = 0; i < NPAIR; i++) {
-                                uint32_t v[32];
-                                tmem_ld32(tmem + lanes + i * AK_HEADS + 32 * hf, v);
-                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                                for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * f[k]);
-                                tmem_st32(tmem + lanes + i * AK_HEADS + 32 * hf, v);
+                            for (int k = 0; k < 8; k++) {
+                                const float4 g = f[k];
+                                s[4 * k] = __float_as_uint(__uint_as_float(s[4 * k]) * g.x);
+                                s[4 * k + 1] = __float_as_uint(__uint_as_float(s[4 * k + 1]) * g.y);
+                                s[4 * k + 2] = __float_as_uint(__uint_as_float(s[4 * k + 2]) * g.z);
+                                s[4 * k + 3] = __float_as_uint(__uint_as_float(s[4 * k + 3]) * g.w);
                             }
+                            tmem_st32(o, s);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tmem_ld32(tmem_s + lanes + hh, s);               // again: registers are few
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     }
                 }
+                // all references before the first store: a load behind a store waits for it to issue, one piece after another
+                float4 m[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) m[i] = mp[i];
                 uint32_t top = 0;                        // the largest numerator: as BF16 bits they compare like numbers
-#pragma unroll 1
-                for (int hf = 0; hf < 2; hf++) {
-                    uint32_t s[32];
-                    tmem_ld32(tmem_s + lanes + 32 * hf, s);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    // all references before the first store: a load behind a store waits for it to issue, one piece after another
-                    // (64 columns 1,200 cycles; 650 so, of which the exponentials need 512)
-                    float4 m[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) m[i] = mp[8 * hf + i];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const int i = 8 * c + 4 * k;
-                            const float4 r = m[2 * c + k];
-                            w[2 * k] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i]), cs, -r.x)), ex2(fmaf(__uint_as_float(s[i + 1]), cs, -r.y)));
-                            w[2 * k + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[i + 3]), cs, -r.w)));
-                            top = max_u16x2(top, max_u16x2(w[2 * k], w[2 * k + 1]));
-                        }
-                        sts16(prow + (((hf * 4 + c) ^ (token & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                    for (int k = 0; k < 2; k++) {
+                        const int i = 8 * c + 4 * k;
+                        const float4 r = m[2 * c + k];
+                        w[2 * k] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i]), cs, -r.x)), ex2(fmaf(__uint_as_float(s[i + 1]), cs, -r.y)));
+                        w[2 * k + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[i + 3]), cs, -r.w)));
+                        top = max_u16x2(top, max_u16x2(w[2 * k], w[2 * k + 1]));
                     }
+                    sts16(prow + ((((hh >> 3) + c) ^ (token & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
                 }
                 // a numerator above 2^AK_SLACK: once more with new references
                 if (!soft_any(max(top & 0xffffu, top >> 16) > (127u + AK_SLACK) << 7) || set) break;
@@ -642,8 +635,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
             mbar_arrive_warp(&sm.p_ready, lane);
             // while the MMAs run: the sums of the numerators, as they were rounded, so that the weights add up to one
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(smem + AK_P_OFF + (lt + k) * 128 + ((lh ^ k) << 4));
+            for (int k = 0; k < 4; k++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(smem + AK_P_OFF + (lt + k) * 128 + ((lh ^ ((lt + k) & 7)) << 4));
                 l[0] += __uint_as_float(w.x << 16); l[1] += __uint_as_float(w.x & 0xffff0000u);
                 l[2] += __uint_as_float(w.y << 16); l[3] += __uint_as_float(w.y & 0xffff0000u);
                 l[4] += __uint_as_float(w.z << 16); l[5] += __uint_as_float(w.z & 0xffff0000u);
@@ -662,7 +655,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
         }
         soft_sync();
         if (tid < AK_HEADS) {
-            const float m = sm.m[tid], sum = (sm.part[0][tid] + sm.part[1][tid]) + (sm.part[2][tid] + sm.part[3][tid]);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < AK_SOFT; i++) sum += sm.part[i][tid];
+            const float m = sm.m[tid];
             if (C > 1) reinterpret_cast<float2 *>(part + AK_HEADS * a.d)[tid] = make_float2(m, sum);
             // the only CTA of its row: what its part is multiplied by, while the last MMAs run
             const float sk = sink * LOG2E, top = fmaxf(sk, m), den = ex2(sk - top) + sum * ex2(m - top);
@@ -741,7 +737,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8)
+    if (warp == AK_MMA)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
