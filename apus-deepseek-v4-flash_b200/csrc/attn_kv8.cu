@@ -175,6 +175,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
           "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
+}
 // kind::f16, BF16 operands, f32 sums, 128 x 64 x 16; `mn`: both operands MN-major
 __device__ __forceinline__ uint32_t ak_idesc(bool mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (mn ? (1u << 15) | (1u << 16) : 0u) | ((uint32_t)(AK_HEADS >> 3) << 17) |
@@ -679,36 +685,33 @@ attn_kv8_kernel(const AttnKv8Args a) {
     if (warp < 16 && (any || C == 1)) {
         const int quad = warp & 3, hh = (warp >> 2 & 1) * 32;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const float4 *f = reinterpret_cast<const float4 *>(sm.f + hh);
+        const int heads = min(nh - hh, 32), item = C == 1 && a.o_bf16 ? 2 : 4;
+        // 16 heads at a time and not 32: half the code, which has to be fetched for few rounds of it
 #pragma unroll 1
-        for (int i = warp >> 3; i < NPAIR; i += 2) {
-            const int ch0 = i * 128 + quad * 32;
-            if (ch0 >= a.d) break;
-            const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane);     // panels of codes have an order of their own
-            uint32_t v[32];
-            if (any) {
-                tmem_ld32(tmem + lanes + i * AK_HEADS + hh, v);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            }
-            if (C > 1) {
-                float *p = part + hh * a.d + ch;
+        for (int k0 = 0; k0 < heads; k0 += 16) {
+            float f[16];
 #pragma unroll
-                for (int k = 0; k < 32; k++, p += a.d)
-                    if (hh + k < nh) __stcg(p, __uint_as_float(v[k]));
-                continue;
-            }
-            // the output's rows in shared memory, a warp's 32 channels of a head at a time
-            const uint32_t base = smem_u32(smem) + (hh * a.d + ch) * (a.o_bf16 ? 2 : 4), step = a.d * (a.o_bf16 ? 2 : 4);
+            for (int k = 0; k < 16; k++) f[k] = sm.f[hh + k0 + k];
+#pragma unroll 1
+            for (int i = warp >> 3; i < NPAIR; i += 2) {
+                const int ch0 = i * 128 + quad * 32;
+                if (ch0 >= a.d) break;
+                const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane); // panels of codes have an order of their own
+                uint32_t v[16];
+                if (any) tmem_ld16(tmem + lanes + i * AK_HEADS + hh + k0, v);
+                if (C > 1) {
+                    float *p = part + (hh + k0) * a.d + ch;
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-                const float4 g = f[k / 4];
-                const float x[4] = {__uint_as_float(v[k]) * g.x, __uint_as_float(v[k + 1]) * g.y, __uint_as_float(v[k + 2]) * g.z,
-                                    __uint_as_float(v[k + 3]) * g.w};
+                    for (int k = 0; k < 16; k++, p += a.d)
+                        if (k0 + k < heads) __stcg(p, __uint_as_float(v[k]));
+                } else {                                 // the output's rows in shared memory, a warp's 32 channels of a head at a time
+                    const uint32_t base = smem_u32(smem) + ((hh + k0) * a.d + ch) * item, step = a.d * item;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t u = any ? bf16x2_rn(0.f, x[j]) : 0u;
-                    if (a.o_bf16) asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + (k + j) * step), "h"((uint16_t)(u >> 16)));
-                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + (k + j) * step), "r"(u));
+                    for (int k = 0; k < 16; k++) {
+                        const uint32_t u = any ? bf16x2_rn(0.f, __uint_as_float(v[k]) * f[k]) : 0u;
+                        if (a.o_bf16) asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + k * step), "h"((uint16_t)(u >> 16)));
+                        else asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + k * step), "r"(u));
+                    }
                 }
             }
         }
