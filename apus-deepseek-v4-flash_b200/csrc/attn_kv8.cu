@@ -26,6 +26,7 @@ struct AttnKv8Args {
     float scale;
     int q_bf16, o_bf16;
     int cluster, unit;           // CTAs per query row, tokens per tile (a multiple of 16 up to 112)
+    int ahead;                   // rows that the GPU works on at once
     float *part;                 // [CTA]: O^T of a part as [64][d], then its 64 references and sums; where a row has several CTAs
     int *status;
 };
@@ -88,16 +89,22 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 //
 // A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA
 // writes its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts
-// of its share of the heads in rank order: one launch, the same bits every time.  Through L2 and not through distributed
-// shared memory, which moves 15 bytes a cycle into an SM however it is asked (128 KB took 13,000 cycles; so 6,000).
+// of its share of the heads in rank order: one launch, the same bits every time.  Through L2, which takes 3,300 cycles
+// to write and 3,200 to 6,800 to read 128 KB per SM; distributed shared memory moved 15 bytes a cycle into an SM, 8,700 cycles.
 //
-// Warps 0 to 3: softmax.  Warps 4 to 17: rows, fetched into registers a tile ahead and dequantised into shared memory, the
-// first seven of them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one
-// dequantises.  Warp 18 issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64
-// heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
+// Warps 0 to 7: softmax, two threads per token, 32 heads each (one thread with all 64: the numerators 500 cycles later, a tile
+// 4 % slower).  Warps 8 to 21: rows, fetched into registers a tile ahead and dequantised into shared memory, the first seven of
+// them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one dequantises.  Warp 22
+// issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64 heads x 64
+// channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
 // shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
 // TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
 // comes of them is masked.)
+//
+// A tile takes 6,300 cycles.  In 4,000 of them shared memory is busy: 60 MMAs read 6 KB each at 128 bytes a cycle, and the rows'
+// 112 KB are written while the MMAs of the tile before, panel pair by panel pair, leave their place.  In the other 2,000 the
+// tensor cores wait for the numerators.  (Two tiles of 64 and 48 tokens in turn, the one's scores under the other's softmax, took
+// 7,300: an instruction of 64 rows takes as long as one of 128.)
 constexpr int AK_TILE = 112, AK_HEADS = 64;
 constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
@@ -131,7 +138,7 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // A wait of a whole warp, which goes on together; false when it ran out or another one did.  One loop, not unrolled, like the
 // others below: this kernel's roles run through their code once per tile, and what the instruction caches do not hold they
-// wait for (124 KB of code, half of it unrolled waits, took 20 % longer than 60 KB).
+// wait for.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t addr = smem_u32(bar);
     unsigned long long t0 = 0;
@@ -479,6 +486,13 @@ attn_kv8_kernel(const AttnKv8Args a) {
         const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
         const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
         const uint64_t dv = ak_desc_mn(smem_u32(smem)), dp = ak_desc_mn(smem_u32(smem + AK_P_OFF));
+        // The queries of the row that a later CTA on this SM may have, into L2 (1,024 rows of 640 candidates: 209 us without, 206 with)
+        if (rank == 0 && lane == 0 && row + (uint32_t)a.ahead < (uint32_t)a.rows) {
+            const uint32_t item = a.q_bf16 ? 2u : 4u;
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                         ::"l"(static_cast<const uint8_t *>(a.q) + ((size_t)(row + a.ahead) * a.h + h0) * a.d * item), "r"((uint32_t)nh * a.d * item) : "memory");
+        }
+        __syncwarp();
         if (!warp_wait(&sm.q_full, 0u, s_abort)) fail = 51;
         while (more) {
             const int ks = (min(a.unit, a.idxw - tile * a.unit) + 15) >> 4;      // steps of 16 tokens that hold any
@@ -747,8 +761,16 @@ attn_kv8_kernel(const AttnKv8Args a) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// CTAs per query row, and tokens per tile.  `slots`: clusters of 1, 2, 4, 8 and 16 CTAs that the GPU holds at once.
-void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluster, int *unit) {
+// CTAs per query row, and tokens per tile.  `slots`: clusters of 1, 2, 4, 8 and 16 CTAs that the GPU holds at once (148, 74, 33,
+// 15 and 7).  The time in microseconds, fitted to measurements: 9.5 for a CTA's start and end, the join, and 3.15 for a tile of 112
+// tokens, times the turns in which the GPU takes the rows.  Measured, 1 / 2 / 4 / 8 / 16 CTAs per row, * where the rule goes:
+//   1 row of 640 candidates    27.3    22.4     18.2    15.0    14.8*
+//   32 of 640                  29.8    25.1     21.1*   45.8    76.2
+//   48 of 640                  31      25.3*    39      62     107
+//   1 of 8,320                247     134       74      44      30.1*
+//   32 of 8,320               259     140       80.9*  135     151
+//   5 of 128                   13.7    13.5     13.6    13.2*   13.4
+void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluster, int *unit, int *ahead) {
     double best = 0;
     *cluster = 1;
     *unit = 16;
@@ -757,9 +779,9 @@ void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluste
         if (slots[i] < 1 || (i && rows << i > AK_MOST_PARTS)) continue;
         const int k = idxw > AK_TILE * C ? (idxw + AK_TILE * C - 1) / (AK_TILE * C) : 1;      // tiles of the CTA with the most
         const int u = idxw ? ((idxw + C * k - 1) / (C * k) + 15) & ~15 : 16;
-        const double waves = (double)((rows + slots[i] - 1) / slots[i]);
-        const double t = waves * (3.0 + (C > 1 ? 2.0 : 0.0) + k * (1.0 + u / 112.0 * 1.5));
-        if (i == 0 || t < best) { best = t; *cluster = C; *unit = u; }
+        const double turns = (double)((rows + slots[i] - 1) / slots[i]);
+        const double t = turns * (9.5 + (C > 1 ? 2.5 + 0.05 * C : 0.0) + k * (1.25 + u / 112.0 * 1.9));
+        if (i == 0 || t < best) { best = t; *cluster = C; *unit = u; *ahead = slots[i]; }
     }
 }
 
@@ -800,7 +822,7 @@ int attn_kv8(AttnKv8Args a, cudaStream_t st) {
     a.status = wait_word();
     if (!dev || !a.status) return 1;
     const unsigned hb = (unsigned)ceil_div(a.h, AK_HEADS);
-    attn_kv8_shape(a.idxw, (long long)a.rows * hb, dev->slots[a.rd != 0], &a.cluster, &a.unit);
+    attn_kv8_shape(a.idxw, (long long)a.rows * hb, dev->slots[a.rd != 0], &a.cluster, &a.unit, &a.ahead);
     CallScratch scratch(st);
     if (a.cluster > 1 && scratch.get((size_t)a.rows * hb * a.cluster * (AK_HEADS * a.d + 2 * AK_HEADS) * sizeof(float))) return 1;
     a.part = static_cast<float *>(scratch.p);
@@ -843,6 +865,6 @@ extern "C" int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const fl
     APUS_REQUIRE(aligned16(q) && aligned16(o), "sparse_attn_kv8: queries and output must start on a 16-byte boundary");
     if (ensure_enabled()) return 1;
     const AttnKv8Args a = {q, sink, idxs, kv_a, kv_b, o, na, nb, kv_a_stride, kv_b_stride, h, d, rd, idxw, rows, rows_per_seq,
-                           scale, q_bf16 != 0, o_bf16 != 0, 1, 16, nullptr, nullptr};
+                           scale, q_bf16 != 0, o_bf16 != 0, 1, 16, 0, nullptr, nullptr};
     return attn_kv8(a, (cudaStream_t)stream);
 }
