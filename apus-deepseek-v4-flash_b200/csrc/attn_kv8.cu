@@ -161,11 +161,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -582,24 +577,18 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 tmem_ld32(tmem_s + lanes + hh, s);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (set) {
-                    // New references: the maxima over the tokens so far, as BF16 (they need not be exact), two heads in a register
-                    // and folded over the lanes, after which lane i has those of heads 2 i and 2 i + 1 of this warp's.
-                    uint32_t x[16];
+                    // New references from the maxima over the tokens so far, folded over the lanes, after which lane i has that of
+                    // this warp's head i.
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const uint32_t u = bf16x2_rn(__uint_as_float(s[2 * i]) * cs, __uint_as_float(s[2 * i + 1]) * cs);
-                        x[i] = (u & mask) | (0xff80ff80u & ~mask);
-                    }
+                    for (int i = 0; i < 32; i++) s[i] = (__float_as_uint(__uint_as_float(s[i]) * cs) & mask) | (0xff800000u & ~mask);
 #pragma unroll
-                    for (int o = 8; o; o >>= 1)
+                    for (int o = 16; o; o >>= 1)
 #pragma unroll
                         for (int i = 0; i < o; i++) {
                             const bool up = lane & o;
-                            x[i] = max_bf16x2(up ? x[i + o] : x[i], __shfl_xor_sync(0xffffffffu, up ? x[i] : x[i + o], o));
+                            s[i] = __float_as_uint(fmaxf(__uint_as_float(up ? s[i + o] : s[i]), __uint_as_float(__shfl_xor_sync(0xffffffffu, up ? s[i] : s[i + o], o))));
                         }
-                    x[0] = max_bf16x2(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
-                    if (lane < 16)
-                        *reinterpret_cast<float2 *>(&sm.part[quad][hh + 2 * lane]) = make_float2(__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u));
+                    sm.part[quad][hh + lane] = __uint_as_float(s[0]);
                     soft_sync();
                     if (tid < AK_HEADS) {
                         const float old = sm.m[tid];
@@ -628,9 +617,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
                             tmem_st32(o, s);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        tmem_ld32(tmem_s + lanes + hh, s);               // again: registers are few
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     }
+                    tmem_ld32(tmem_s + lanes + hh, s);   // again: registers are few
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 }
                 // all references before the first store: a load behind a store waits for it to issue, one piece after another
                 float4 m[8];
@@ -731,6 +720,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
         }
     }
     if (C > 1) {
+        // the other CTAs of a row must not join what a wait that ran out has left
+        if (tid < AK_HEADS && *s_abort) reinterpret_cast<float2 *>(part + AK_HEADS * a.d)[tid] = make_float2(NAN, NAN);
         __syncwarp();
         cluster_arrive();
         cluster_wait();                                  // the parts of all CTAs are written
@@ -854,7 +845,7 @@ extern "C" int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const fl
                                              const uint8_t *kv_b, int64_t nb, int64_t kv_b_stride, void *o, int o_bf16, void *stream) {
     if (kv8_check_row("sparse_attn_kv8", d, rd)) return 1;
     APUS_REQUIRE(h > 0 && h <= 1024, "sparse_attn_kv8: h=%d must be 1 to 1024", h);
-    APUS_REQUIRE(rows >= 0 && idxw >= 0, "sparse_attn_kv8: %d rows of %d ids", rows, idxw);
+    APUS_REQUIRE(rows >= 0 && idxw >= 0 && idxw <= 1 << 30, "sparse_attn_kv8: %d rows of %d ids", rows, idxw);
     APUS_REQUIRE(rows_per_seq > 0 && rows % rows_per_seq == 0, "sparse_attn_kv8: %d rows are not sequences of %d", rows, rows_per_seq);
     APUS_REQUIRE(na >= 0 && nb >= 0 && na + nb <= INT32_MAX, "sparse_attn_kv8: na=%lld, nb=%lld", (long long)na, (long long)nb);
     APUS_REQUIRE(kv_a_stride >= 0 && kv_b_stride >= 0, "sparse_attn_kv8: negative stride");

@@ -61,7 +61,7 @@ kv8_write_kernel(const void *x, int d, int rd, uint32_t rows, uint32_t s, const 
     }
     const uint32_t b = row / s;
     const int t = (int)(row - b * s), n = counts ? min(max(counts[b], 0), (int)s) : (int)s;
-    long long at = pos[b] + t;
+    long long at = (long long)((unsigned long long)pos[b] + t);          // beyond the last of all numbers: a negative one
     if (t >= n || at < 0 || (ring ? (long long)n - t > cap : at >= cap)) return;
     if (at >= cap) at = (uint64_t)(at | cap) >> 32 ? at % cap : (uint32_t)at % (uint32_t)cap;
     uint8_t *rec = cache + (size_t)(b * stride + at) * kv8_row_bytes(d, rd);
@@ -114,7 +114,7 @@ kv8_read_kernel(const uint8_t *cache, int d, int rd, long long cap, long long st
     if (row >= rows) return;
     const int lane = threadIdx.x & 31, nq = d - rd;
     const uint32_t b = row / s;
-    const long long e = idx ? (long long)idx[row] : first + (row - b * s);
+    const long long e = idx ? (long long)idx[row] : (long long)((unsigned long long)first + (row - b * s));
     const bool there = e >= 0 && e < cap;
     const uint8_t *rec = cache + (size_t)(there ? b * stride + e : 0) * kv8_row_bytes(d, rd);
     uint4 raw[KV8_STEPS];

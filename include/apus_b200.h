@@ -521,9 +521,8 @@ int apus_cuda_sparse_attn_batch_dev(const float *q, const float *sink, int h, in
  * or 64, below d (0 bytes and a message otherwise).
  * A cache is the caller's device memory: n_seq sequences of `cap` records, sequence b from record
  * b * stride on.  All pointers are device pointers; caches, queries and outputs start on 16-byte
- * boundaries, f32 rows that are written or read on 32-byte ones.  Work is enqueued on `stream`,
- * nothing is kept between calls and no memory is allocated, so calls may run side by side and be
- * recorded into graphs. */
+ * boundaries, f32 rows that are written or read on 32-byte ones.  Work is enqueued on `stream`;
+ * calls may run side by side on several streams and be recorded into graphs. */
 size_t apus_cuda_kv8_row_bytes(int d, int rd);
 /* Quantises x [n_seq, s, d] (f32, or BF16 when x_bf16) into the caches: row t of sequence b goes to
  * entry pos[b] + t (pos [n_seq], on the device), modulo cap when `ring`.  counts [n_seq]
@@ -548,7 +547,11 @@ int apus_cuda_kv8_read_dev(const uint8_t *cache, int d, int rd, int64_t cap, int
  * of holes.  Strides in records (0: one cache for all sequences).  The contractions run on the tensor
  * cores (BF16 products, f32 sums in their order) and the softmax numerators are BF16 as in
  * c/attn.h:1308, so a result is within a BF16 step or two of the reference's, not its bits.  The
- * same call gives the same bits. */
+ * same call gives the same bits; how many SMs share a row, and with it the order of the sums,
+ * follows from rows, h and idxw.  Where several do, the call uses a scratch buffer of the library
+ * that belongs to its stream (at most 135 MB), one that is being recorded gets memory that its
+ * graph owns.  Values of rows below 2^-78 may count as zero.  h: up to 1,024; idxw: up to 2^30;
+ * na + nb < 2^31. */
 int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const float *sink, int h, int d,
                                   int rd, const int32_t *idxs, int idxw, int rows,
                                   int rows_per_seq, float scale, const uint8_t *kv_a, int64_t na,

@@ -338,6 +338,46 @@ def test_scores_far_apart(n, order):
     c.check(c.out())
 
 
+@pytest.mark.parametrize("n,sign", [(1, 1), (120, 1), (120, -1), (700, 1), (700, -1)])
+def test_scores_of_hundreds_of_thousands(n, sign):
+    """Every score is exact and a thousand or more away from the next one, so that the result is the row of the largest one."""
+    c = Case(41, n=n, holes=0.0, na=0, nb=128)
+    x = rows_flat(np.random.default_rng(9), 1, 128, 512)
+    x[0, :, 500] = 1 + np.arange(128) / 128.0               # BF16 holds these, and 1,024 powers of e times them are apart
+    c.kv_b = write_rows(bf16_value(bf16_bits(x.astype(np.float32))), 64)
+    c.q[:] = 0
+    c.q[:, :, 500] = sign * 2.0 ** 10 * 2.0 ** (np.arange(64) % 8)
+    c.scale = 2.0 ** 7
+    c.idx[0] = np.random.default_rng(5).integers(0, 128, n)
+    got = c.out()
+    best = c.idx[0].max() if sign > 0 else c.idx[0].min()
+    row = np.broadcast_to(read_rows(c.kv_b[0, best], 512, 64), got.shape)    # BF16 values
+    if sign > 0:
+        assert np.array_equal(got, row)
+    else:                                                     # the sink is far above every score
+        assert not got.any()
+    c.sink = None
+    assert np.array_equal(c.out(), row)
+
+
+def test_ends_of_the_numbers():
+    """Positions whose rows run past the largest number are dropped, an id list may be as long as the sizes allow."""
+    import torch
+    x = rows(np.random.default_rng(3), 1, 6, 128)
+    cache, xd = torch.zeros(1, 8, 208, dtype=torch.uint8, device="cuda"), dev(x)
+    for pos, ring in (((1 << 63) - 3, 0), ((1 << 63) - 3, 1), (-(1 << 63), 1)):
+        cache.zero_()
+        ok(lib().apus_cuda_kv8_write_dev(ptr(xd), 0, 128, 64, 1, 6, ptr(dev(np.array([pos], np.int64))), None, ring, ptr(cache), 8, 8, stream()), "kv8_write")
+        got, want = cache.cpu().numpy(), np.zeros((1, 8, 208), np.uint8)
+        if pos > 0 and ring:
+            for t in range(3):
+                want[0, (pos + t) % 8] = write_rows(x, 64)[0, t]
+        assert same(got, want)
+    out = torch.full((1, 6, 128), 3.0, device="cuda")
+    ok(lib().apus_cuda_kv8_read_dev(ptr(cache), 128, 64, 8, 8, 1, 6, None, (1 << 63) - 3, ptr(out), 0, stream()), "kv8_read")
+    assert not out.any()
+
+
 def test_large_and_small_rows():
     """Scale bytes up to the largest that BF16 holds the values of, and down to the smallest that is written."""
     c = Case(11, n=100, holes=0.0, nb=60, na=0)

@@ -46,7 +46,7 @@ def test_read(change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(h=0), "h="), (dict(h=1025), "h="), (dict(rows=-1), "rows"), (dict(idxw=-1), "ids"), (dict(per=0), "sequences"), (dict(per=4), "sequences"),
+    (dict(h=0), "h="), (dict(h=1025), "h="), (dict(rows=-1), "rows"), (dict(idxw=-1), "ids"), (dict(idxw=(1 << 30) + 1), "ids"), (dict(per=0), "sequences"), (dict(per=4), "sequences"),
     (dict(na=-1), "na="), (dict(nb=-1), "nb="), (dict(nb=1 << 31), "nb="), (dict(sa=-1), "stride"), (dict(sb=-1), "stride"), (dict(kv_a=None), "no cache"),
     (dict(kv_b=None), "no cache"), (dict(kv_a=CACHE + 8), "16-byte"), (dict(kv_b=CACHE + 4), "16-byte"), (dict(q=None), "queries"), (dict(o=None), "output"),
     (dict(idxs=None), "ids"), (dict(q=X + 4), "16-byte"), (dict(o=OUT + 2), "16-byte")])
