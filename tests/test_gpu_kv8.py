@@ -446,6 +446,105 @@ def test_streams_graphs_and_repeats_give_the_same_bits():
     del graph
 
 
+@pytest.mark.parametrize("n,h,rows,per", [(300, 130, 200, 50), (40, 1024, 20, 20), (700, 1000, 2, 1)])
+def test_many_heads_and_more_rows_than_the_gpu_holds(n, h, rows, per):
+    c = Case(h, h=h, n=n, seqs=rows // per, per=per, nb=300)
+    got = c.out()
+    c.check(got, [0, rows // 2, rows - 1])
+
+
+@pytest.mark.parametrize("n", [100, 700])
+@pytest.mark.parametrize("out_bf16", [False, True])
+def test_pointers_on_16_byte_boundaries_only(n, out_bf16):
+    """Queries, caches and output 16 bytes behind a coarser boundary, the bytes around the output as they were."""
+    import torch
+    c = Case(51, n=n, seqs=3, h=33)
+    want = c.out(bf16=out_bf16)
+    def shifted(t):
+        raw = torch.zeros(t.numel() * t.element_size() + 4096, dtype=torch.uint8, device="cuda")
+        at = (-raw.data_ptr()) % 1024 + 16
+        v = raw[at:at + t.numel() * t.element_size()]
+        v.copy_(t.reshape(-1).view(torch.uint8))
+        return raw, v
+    keep = [shifted(t) for t in (c.dq, c.da, c.db)]
+    c.dq, c.da, c.db = (v for _, v in keep)
+    es = 2 if out_bf16 else 4
+    raw = torch.full((c.rows * c.h * c.d * es + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    at = (-raw.data_ptr()) % 1024 + 16
+    o = raw[at:at + c.rows * c.h * c.d * es].view(torch.bfloat16 if out_bf16 else torch.float32)
+    ok(c.call(o), "attn")
+    assert same(o.float().cpu().numpy().reshape(want.shape), want)
+    assert (raw[:at] == 0x5A).all() and (raw[at + o.numel() * es:] == 0x5A).all()
+
+
+def test_graphs_and_threads_side_by_side():
+    """Two graphs whose rows are shared by several SMs, replayed on two streams at once, while two threads call on a third stream
+    and on one each, with sizes that make the scratch of a stream grow."""
+    import threading
+    import torch
+    cases = [Case(60 + i, n=n, seqs=s).put() for i, (n, s) in enumerate([(640, 2), (1500, 5), (300, 1), (2500, 9)])]
+    want = []
+    for c in cases:
+        o = torch.empty(c.rows, c.h, c.d, device="cuda")
+        ok(c.call(o), "attn")
+        want.append(o)
+    streams = [torch.cuda.Stream() for _ in range(5)]
+    graphs, outs = [], [torch.empty_like(w) for w in want[:2]]
+    for c, o, s in zip(cases, outs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ok(c.call(o, s.cuda_stream), "attn")
+        graphs.append(g)
+    torch.cuda.synchronize()
+    got, rcs = [[], []], []
+
+    def calls(k):
+        for i in range(12):
+            c, w = cases[(i + k) % 4], want[(i + k) % 4]
+            s = streams[2] if i & 1 else streams[3 + k]
+            with torch.cuda.stream(s):
+                o = torch.empty_like(w)
+            rcs.append(c.call(o, s.cuda_stream))
+            got[k].append((o, w))
+
+    ts = [threading.Thread(target=calls, args=(k,)) for k in range(2)]
+    for t in ts:
+        t.start()
+    for _ in range(12):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    for t in ts:
+        t.join()
+    torch.cuda.synchronize()
+    assert not any(rcs)
+    for o, w in [*got[0], *got[1], *zip(outs, want)]:
+        assert torch.equal(o, w)
+    del graphs
+
+
+def test_the_first_call_of_a_process_may_be_recorded():
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = %r
+import numpy as np, torch
+from test_gpu_kv8 import Case, lib, ok
+c = Case(3, n=640, seqs=2).put()
+o = torch.zeros(2, 64, 512, device="cuda")
+g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=s):
+    ok(c.call(o, s.cuda_stream), "attn")
+g.replay()
+torch.cuda.synchronize()
+c.check(o.cpu().numpy())
+""" % (sys.path,)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_a_decode_loop_over_8_bit_caches_is_the_loop_over_bf16_rows():
     """Written, attended and read back as a token loop does: a ring of the last positions and a cache that grows by an entry
     every few of them, beside apus_cuda_sparse_attn_batch_dev over the same rows in BF16."""
