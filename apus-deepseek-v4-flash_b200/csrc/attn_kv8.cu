@@ -75,8 +75,8 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 //   S^T[token, head]   = K[token, ch] Q[head, ch]^T     A = 128 rows as they lie (K-major),  B = the queries
 //   O^T[ch, head]     += V[token, ch]^T P[token, head]   A = the same rows (MN-major),         B = the numerators
 //
-// With tokens, then channels as the 128 rows of an instruction, the 64 heads are its columns and no instruction runs half
-// empty.  A group of codes times its power of two is a BF16 value exactly (4 significant bits), so nothing is rounded
+// With tokens, then channels as the 128 rows of an instruction, the heads are its columns (64, 32 or 16 in a CTA:
+// attn_kv8_shape) and no instruction runs half empty.  A group of codes times its power of two is a BF16 value exactly (4 significant bits), so nothing is rounded
 // before the products.  A token is a TMEM lane, so that a thread turns one token's scores into numerators for 32 heads and
 // stores them as one contiguous piece of a row of P.
 //
@@ -92,24 +92,22 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // of its share of the heads in rank order: one launch, the same bits every time.  Through L2, which takes 3,300 cycles
 // to write and 3,200 to 6,800 to read 128 KB per SM; distributed shared memory moved 15 bytes a cycle into an SM, 8,700 cycles.
 //
-// Warps 0 to 7: softmax, two threads per token, 32 heads each (one thread with all 64: the numerators 500 cycles later, a tile
-// 4 % slower).  Warps 8 to 21: rows, fetched into registers a tile ahead and dequantised into shared memory, the first seven of
+// Warps 0 to 7: softmax, two threads per token, half of the heads each (one thread with all 64: the numerators 500 cycles later,
+// a tile 4 % slower).  Warps 8 to 21: rows, fetched into registers a tile ahead and dequantised into shared memory, the first seven of
 // them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one dequantises.  Warp 22
-// issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of 64 heads x 64
-// channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
+// issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of the
+// heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
 // shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
 // TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
 // comes of them is masked.)
 //
-// A tile takes 6,300 cycles.  In 4,000 of them shared memory is busy: 60 MMAs read 6 KB each at 128 bytes a cycle, and the rows'
+// A tile takes 6,300 cycles with 64 heads (5,700 with 32, 5,400 with 16).  In 4,000 of them shared memory is busy: 60 MMAs read 6 KB each at 128 bytes a cycle, and the rows'
 // 112 KB are written while the MMAs of the tile before, panel pair by panel pair, leave their place.  In the other 2,000 the
 // tensor cores wait for the numerators.  (Two tiles of 64 and 48 tokens in turn, the one's scores under the other's softmax, took
 // 7,300: an instruction of 64 rows takes as long as one of 128.)
-constexpr int AK_TILE = 112, AK_HEADS = 64;
+constexpr int AK_TILE = 112, AK_HEADS = 64;             // of the largest CTA
 constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
-constexpr int AK_PANEL = AK_TILE * 128, AK_QPANEL = AK_HEADS * 128;
-constexpr int AK_ASK = (AK_HEADS * KV8_MAX_D / 8 + 32 * AK_MMA - 1) / (32 * AK_MMA);             // pieces of 8 query channels per thread
-constexpr int AK_Q_OFF = 8 * AK_PANEL, AK_P_OFF = AK_Q_OFF + 8 * AK_QPANEL, AK_MISC_OFF = AK_P_OFF + 128 * 128;
+constexpr int AK_PANEL = AK_TILE * 128, AK_Q_OFF = 8 * AK_PANEL;
 constexpr int AK_MOST_PARTS = 1024;                     // 135 MB of scratch
 constexpr uint32_t AK_SLACK = 64;                       // as values of rows go up to 2^16, the f32 sums hold 2^40 such products
 constexpr float AK_ABOVE = 48.f, AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
@@ -122,9 +120,19 @@ struct AkMisc {
     uint32_t tmem;
     int abort;
 };
-constexpr int AK_SMEM = AK_MISC_OFF + (int)sizeof(AkMisc);
-static_assert(AK_SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
-static_assert(AK_HEADS * KV8_MAX_D * 4 <= AK_P_OFF, "the output as f32 in the place of panels and queries");
+// What depends on the heads of a CTA.
+template <int H>
+struct Ak {
+    static constexpr int ASK = (H * KV8_MAX_D / 8 + 32 * AK_MMA - 1) / (32 * AK_MMA);   // pieces of 8 query channels per thread
+    static constexpr int W = H / 2;                      // heads of a softmax thread
+    static constexpr int QPANEL = H * 128, P_OFF = AK_Q_OFF + 8 * QPANEL, P_ROW = H * 2, MISC_OFF = P_OFF + 128 * P_ROW;
+    static constexpr int SMEM = MISC_OFF + (int)sizeof(AkMisc);
+    static constexpr int COLUMNS = H == 64 ? 512 : H == 32 ? 256 : 128;                 // of tensor memory: 4 H of O^T, H of S^T
+    // a row of P fills 128, 64 or 32 bytes and is swizzled as wide: its 16-byte pieces by these bits of its address
+    static __device__ __forceinline__ int p_swizzle(int token) { return (token * P_ROW >> 7) & (H / 8 - 1); }
+    static_assert(SMEM <= 195 * 1024, "shared memory that leaves 60 KB of L1");
+    static_assert(H * KV8_MAX_D * 4 <= P_OFF, "the output as f32 in the place of panels and queries");
+};
 
 // barriers of the softmax warps
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -166,7 +174,18 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void ak_ld(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void ak_ld(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void ak_ld(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void ak_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ak_st(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
         "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -177,15 +196,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
           "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
+__device__ __forceinline__ void ak_st(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                   "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-// kind::f16, BF16 operands, f32 sums, 128 x 64 x 16; `mn`: both operands MN-major
-__device__ __forceinline__ uint32_t ak_idesc(bool mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (mn ? (1u << 15) | (1u << 16) : 0u) | ((uint32_t)(AK_HEADS >> 3) << 17) |
+__device__ __forceinline__ void ak_st(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+// kind::f16, BF16 operands, f32 sums, 128 x heads x 16; `mn`: both operands MN-major
+__device__ __forceinline__ uint32_t ak_idesc(int heads, bool mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (mn ? (1u << 15) | (1u << 16) : 0u) | ((uint32_t)(heads >> 3) << 17) |
            ((uint32_t)(128 >> 4) << 24);
 }
 // Issued by one lane of a whole, converged warp: with no branch around it the descriptors stay in uniform registers.
@@ -204,10 +226,10 @@ __device__ __forceinline__ void ak_commit(uint64_t *bar) {
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
         ::"r"(smem_u32(bar)) : "memory");
 }
-// MN-major operand of 128-byte swizzled rows, a row per k: 64 elements of M or N in a row, the next 64 a panel further
-__device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(AK_PANEL >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
+// MN-major operand, a row of `width` bytes per k, swizzled as wide (128, 64 or 32); where M goes on, a panel further
+__device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr, int width) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(AK_PANEL >> 4) << 16 | (uint64_t)(8 * width >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)(width == 128 ? 2 : width == 64 ? 4 : 6) << 61;
 }
 
 // Where a channel of a panel of codes lies (codes_bf16x4): queries and output channels follow it.
@@ -312,9 +334,9 @@ struct TileRows {
 // The parts of a row's C CTAs, joined for this CTA's share of the heads: U times 4 channels of a head and R of the parts at a
 // time, eight loads in flight
 template <int U, int R>
-__device__ __forceinline__ void ak_join(int C, float *w, const float *parts, int d, const float *sink, void *o, int o_bf16, int rank, int nh) {
+__device__ __forceinline__ void ak_join(int C, int H, float *w, const float *parts, int d, const float *sink, void *o, int o_bf16, int rank, int nh) {
     const int per = (nh + C - 1) / C, lo = rank * per, n = min(per, nh - lo), tid = threadIdx.x;
-    const uint32_t part_size = AK_HEADS * d + 2 * AK_HEADS;
+    const uint32_t part_size = H * d + 2 * H;
     if (tid < AK_HEADS) {
         // lane i of a head's C lanes: reference and sum of part i; w [head][part]: what a part is multiplied by, -1 for one
         // without tokens, which has not been written
@@ -322,7 +344,7 @@ __device__ __forceinline__ void ak_join(int C, float *w, const float *parts, int
         float2 v = make_float2(AK_NONE, 0.f);
         float sk = -INFINITY;
         if (hd < n) {
-            v = __ldcg(reinterpret_cast<const float2 *>(parts + r * part_size + AK_HEADS * d) + lo + hd);
+            v = __ldcg(reinterpret_cast<const float2 *>(parts + r * part_size + H * d) + lo + hd);
             if (sink) sk = sink[lo + hd] * LOG2E;
         }
         float top = fmaxf(v.x, sk);
@@ -374,18 +396,20 @@ __device__ __forceinline__ void ak_join(int C, float *w, const float *parts, int
     }
 }
 
-template <bool TAIL>
+template <bool TAIL, int H>
 __global__ void __launch_bounds__(AK_THREADS, 1)
 attn_kv8_kernel(const AttnKv8Args a) {
     APUS_PDL_GO();
+    using K = Ak<H>;
+    constexpr int W = K::W;
     extern __shared__ __align__(1024) uint8_t smem[];
-    AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + AK_MISC_OFF);
+    AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + K::MISC_OFF);
     volatile int *s_abort = &sm.abort;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, C = a.cluster;
-    const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * AK_HEADS, nh = min(AK_HEADS, a.h - h0);
+    const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * H, nh = min(H, a.h - h0);
     const uint32_t row = blockIdx.x / (unsigned)C, seq = row / (uint32_t)a.rows_per_seq;
     const Kv8Seq at(a, seq);
-    const size_t part_size = AK_HEADS * a.d + 2 * AK_HEADS;
+    const size_t part_size = H * a.d + 2 * H;
     float *part = a.part + (blockIdx.y * (size_t)gridDim.x + blockIdx.x) * part_size;
     const int32_t *ids = a.idxs + (size_t)row * a.idxw;
     const int n_tiles = (a.idxw + a.unit - 1) / a.unit, NP = a.d / 64, NPAIR = (NP + 1) / 2;
@@ -402,7 +426,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < AK_HEADS) sm.m[tid] = AK_NONE;
+    if (tid < H) sm.m[tid] = AK_NONE;
     APUS_PDL_WAIT();
 
     // What the first tile waits for: its ids, sinks, and the queries, 8 channels at a time, all at once, by all warps but the one
@@ -410,14 +434,14 @@ attn_kv8_kernel(const AttnKv8Args a) {
     TileIds cur;                                         // of tile `tile`, which has a record in it while `more`
     int tile = rank;
     cur.load(a, ids, tile, lane);
-    uint4 qv[AK_ASK][2];
+    uint4 qv[K::ASK][2];
     const int per_head = a.d / 8, q_heads = 32 * AK_MMA / per_head, q_rest = 32 * AK_MMA % per_head;
     int q_head = tid / per_head, q_c = tid % per_head;   // of this thread's next piece
     auto ask = [&]() {
         const uint8_t *q = static_cast<const uint8_t *>(a.q) + ((size_t)row * a.h + h0) * a.d * (a.q_bf16 ? 2 : 4);
         int hd = q_head, c = q_c;
 #pragma unroll
-        for (int k = 0; k < AK_ASK; k++) {
+        for (int k = 0; k < K::ASK; k++) {
             const uint8_t *p = q + (uint32_t)((hd < nh ? hd * per_head : 0) + c) * (a.q_bf16 ? 16u : 32u);
             qv[k][0] = ldg16(p);
             if (!a.q_bf16) qv[k][1] = ldg16(p + 16);
@@ -428,7 +452,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     };
     auto place = [&]() {
 #pragma unroll
-        for (int k = 0; k < AK_ASK; k++) {
+        for (int k = 0; k < K::ASK; k++) {
             uint4 v = qv[k][0];
             if (!a.q_bf16)
                 v = make_uint4(bf16x2_rn(__uint_as_float(v.x), __uint_as_float(v.y)), bf16x2_rn(__uint_as_float(v.z), __uint_as_float(v.w)),
@@ -437,7 +461,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
             if (q_c * 8 < a.d - a.rd)                    // in the order of the codes
                 v = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x5410),
                                __byte_perm(v.z, v.w, 0x7632));
-            if (q_head < AK_HEADS) sts16(smem + AK_Q_OFF + (q_c >> 3) * AK_QPANEL + q_head * 128 + (((q_c & 7) ^ (q_head & 7)) << 4), v);
+            if (q_head < H) sts16(smem + AK_Q_OFF + (q_c >> 3) * K::QPANEL + q_head * 128 + (((q_c & 7) ^ (q_head & 7)) << 4), v);
             q_head += q_heads;
             q_c += q_rest;
             if (q_c >= per_head) { q_c -= per_head; q_head++; }
@@ -448,13 +472,13 @@ attn_kv8_kernel(const AttnKv8Args a) {
 
     if (warp == AK_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&sm.tmem)), "r"(512) : "memory");
+                     ::"r"(smem_u32(&sm.tmem)), "r"(K::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0), tmem_s = tmem + 4 * AK_HEADS;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0), tmem_s = tmem + 4 * H;
 
     // A wait that runs out sets the abort flag, after which every other wait gives up soon; all loops and barriers are gone
     // through all the same, so that no thread is left waiting, and nothing is written.
@@ -478,9 +502,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
         mbar_arrive_warp(&sm.q_full, lane);
     }
     if (warp == AK_MMA) {
-        const uint32_t id_s = ak_idesc(false), id_o = ak_idesc(true);
+        const uint32_t id_s = ak_idesc(H, false), id_o = ak_idesc(H, true);
         const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
-        const uint64_t dv = ak_desc_mn(smem_u32(smem)), dp = ak_desc_mn(smem_u32(smem + AK_P_OFF));
+        const uint64_t dv = ak_desc_mn(smem_u32(smem), 128), dp = ak_desc_mn(smem_u32(smem + K::P_OFF), K::P_ROW);
         // The queries of the row that a later CTA on this SM may have, into L2 (1,024 rows of 640 candidates: 209 us without, 206 with)
         if (rank == 0 && lane == 0 && row + (uint32_t)a.ahead < (uint32_t)a.rows) {
             const uint32_t item = a.q_bf16 ? 2u : 4u;
@@ -499,7 +523,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     if (!warp_wait(&sm.full[pn >> 1], done & 1u, s_abort)) fail = 52;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
-                const uint64_t da = dk + pn * (AK_PANEL >> 4), db = dq + pn * (AK_QPANEL >> 4);
+                const uint64_t da = dk + pn * (AK_PANEL >> 4), db = dq + pn * (K::QPANEL >> 4);
                 if (!fail)
 #pragma unroll
                     for (int j = 0; j < 4; j++) ak_mma(tmem_s, da + 2 * j, db + 2 * j, id_s, (pn | j) ? 1u : 0u);
@@ -511,10 +535,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
 #pragma unroll 1
                 for (int i = 0; i < NPAIR; i++) {
                     const uint64_t da = dv + 2 * i * (AK_PANEL >> 4);
-                    ak_mma(tmem + i * AK_HEADS, da, dp, id_o, done ? 1u : 0u);
+                    ak_mma(tmem + i * H, da, dp, id_o, done ? 1u : 0u);
 #pragma unroll
                     for (int k = 1; k < AK_TILE / 16; k++)
-                        if (k < ks) ak_mma(tmem + i * AK_HEADS, da + 128 * k, dp + 128 * k, id_o, 1u);
+                        if (k < ks) ak_mma(tmem + i * H, da + 128 * k, dp + K::P_ROW * k, id_o, 1u);
                     ak_commit(&sm.empty[i]);
                 }
             }
@@ -554,16 +578,17 @@ attn_kv8_kernel(const AttnKv8Args a) {
             done++;
         }
     } else {
-        // a thread has one token and 32 of the heads
-        const int quad = warp & 3, hh = (warp >> 2) * 32, token = tid & 127;
+        // a thread has one token and half of the heads
+        const int quad = warp & 3, hh = (warp >> 2) * W, token = tid & 127;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const float cs = a.scale * LOG2E;
-        // sums of numerators: of 8 heads, over the 4 tokens in a row that this thread adds up of every tile
-        const int lh = tid & 7, lt = (tid >> 3) * 4;
+        // sums of numerators: of 8 heads, over the few tokens in a row that this thread adds up of every tile
+        constexpr int PIECES = H / 8, TOKENS = H / 16;
+        const int lh = tid & (PIECES - 1), lt = tid / PIECES * TOKENS;
         float l[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) l[i] = 0.f;
-        uint8_t *prow = smem + AK_P_OFF + token * 128;
+        uint8_t *prow = smem + K::P_OFF + token * K::P_ROW;
         const float4 *mp = reinterpret_cast<const float4 *>(sm.m + hh);
         while (more) {
             const bool valid = (quad == 0 ? cur.id[0] : quad == 1 ? cur.id[1] : quad == 2 ? cur.id[2] : cur.id[3]) >= 0;
@@ -573,24 +598,27 @@ attn_kv8_kernel(const AttnKv8Args a) {
             if (!warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (bool set = done == 0;; set = true) {
-                uint32_t s[32];
-                tmem_ld32(tmem_s + lanes + hh, s);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                uint32_t s[W];
+                ak_ld(tmem_s + lanes + hh, s);
+                ak_ld_wait();
                 if (set) {
                     // New references from the maxima over the tokens so far, folded over the lanes, after which lane i has that of
                     // this warp's head i.
 #pragma unroll
-                    for (int i = 0; i < 32; i++) s[i] = (__float_as_uint(__uint_as_float(s[i]) * cs) & mask) | (0xff800000u & ~mask);
+                    for (int i = 0; i < W; i++) s[i] = (__float_as_uint(__uint_as_float(s[i]) * cs) & mask) | (0xff800000u & ~mask);
 #pragma unroll
-                    for (int o = 16; o; o >>= 1)
+                    for (int o = W / 2; o; o >>= 1)
 #pragma unroll
                         for (int i = 0; i < o; i++) {
                             const bool up = lane & o;
                             s[i] = __float_as_uint(fmaxf(__uint_as_float(up ? s[i + o] : s[i]), __uint_as_float(__shfl_xor_sync(0xffffffffu, up ? s[i] : s[i + o], o))));
                         }
-                    sm.part[quad][hh + lane] = __uint_as_float(s[0]);
+#pragma unroll
+                    for (int o = W; o < 32; o <<= 1)
+                        s[0] = __float_as_uint(fmaxf(__uint_as_float(s[0]), __uint_as_float(__shfl_xor_sync(0xffffffffu, s[0], o))));
+                    if (lane < W) sm.part[quad][hh + lane] = __uint_as_float(s[0]);
                     soft_sync();
-                    if (tid < AK_HEADS) {
+                    if (tid < H) {
                         const float old = sm.m[tid];
                         const float now = fmaxf(fmaxf(fmaxf(sm.part[0][tid], sm.part[1][tid]), fmaxf(sm.part[2][tid], sm.part[3][tid])) + AK_ABOVE, old);
                         sm.m[tid] = now;
@@ -603,31 +631,31 @@ attn_kv8_kernel(const AttnKv8Args a) {
                         for (int i = 0; i < 8; i++) l[i] *= sm.f[8 * lh + i];
 #pragma unroll 1
                         for (int i = 0; i < NPAIR; i++) {
-                            const uint32_t o = tmem + lanes + i * AK_HEADS + hh;
-                            tmem_ld32(o, s);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            const uint32_t o = tmem + lanes + i * H + hh;
+                            ak_ld(o, s);
+                            ak_ld_wait();
 #pragma unroll
-                            for (int k = 0; k < 8; k++) {
+                            for (int k = 0; k < W / 4; k++) {
                                 const float4 g = f[k];
                                 s[4 * k] = __float_as_uint(__uint_as_float(s[4 * k]) * g.x);
                                 s[4 * k + 1] = __float_as_uint(__uint_as_float(s[4 * k + 1]) * g.y);
                                 s[4 * k + 2] = __float_as_uint(__uint_as_float(s[4 * k + 2]) * g.z);
                                 s[4 * k + 3] = __float_as_uint(__uint_as_float(s[4 * k + 3]) * g.w);
                             }
-                            tmem_st32(o, s);
+                            ak_st(o, s);
                         }
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
-                    tmem_ld32(tmem_s + lanes + hh, s);   // again: registers are few
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    ak_ld(tmem_s + lanes + hh, s);       // again: registers are few
+                    ak_ld_wait();
                 }
                 // all references before the first store: a load behind a store waits for it to issue, one piece after another
-                float4 m[8];
+                float4 m[W / 4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) m[i] = mp[i];
+                for (int i = 0; i < W / 4; i++) m[i] = mp[i];
                 uint32_t top = 0;                        // the largest numerator: as BF16 bits they compare like numbers
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < W / 8; c++) {
                     uint32_t w[4];
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
@@ -637,7 +665,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                         w[2 * k + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[i + 3]), cs, -r.w)));
                         top = max_u16x2(top, max_u16x2(w[2 * k], w[2 * k + 1]));
                     }
-                    sts16(prow + ((((hh >> 3) + c) ^ (token & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                    sts16(prow + ((((hh >> 3) + c) ^ K::p_swizzle(token)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
                 }
                 // a numerator above 2^AK_SLACK: once more with new references
                 if (!soft_any(max(top & 0xffffu, top >> 16) > (127u + AK_SLACK) << 7) || set) break;
@@ -647,8 +675,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
             mbar_arrive_warp(&sm.p_ready, lane);
             // while the MMAs run: the sums of the numerators, as they were rounded, so that the weights add up to one
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(smem + AK_P_OFF + (lt + k) * 128 + ((lh ^ ((lt + k) & 7)) << 4));
+            for (int k = 0; k < TOKENS; k++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(smem + K::P_OFF + (lt + k) * K::P_ROW + ((lh ^ K::p_swizzle(lt + k)) << 4));
                 l[0] += __uint_as_float(w.x << 16); l[1] += __uint_as_float(w.x & 0xffff0000u);
                 l[2] += __uint_as_float(w.y << 16); l[3] += __uint_as_float(w.y & 0xffff0000u);
                 l[4] += __uint_as_float(w.z << 16); l[5] += __uint_as_float(w.z & 0xffff0000u);
@@ -661,17 +689,17 @@ attn_kv8_kernel(const AttnKv8Args a) {
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-            if (lane < 8) sm.part[warp][8 * lane + i] = l[i];
+#pragma unroll
+            for (int o = PIECES; o < 32; o <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+            if (lane < PIECES) sm.part[warp][8 * lane + i] = l[i];
         }
         soft_sync();
-        if (tid < AK_HEADS) {
+        if (tid < H) {
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < AK_SOFT; i++) sum += sm.part[i][tid];
             const float m = sm.m[tid];
-            if (C > 1) reinterpret_cast<float2 *>(part + AK_HEADS * a.d)[tid] = make_float2(m, sum);
+            if (C > 1) reinterpret_cast<float2 *>(part + H * a.d)[tid] = make_float2(m, sum);
             // the only CTA of its row: what its part is multiplied by, while the last MMAs run
             const float sk = sink * LOG2E, top = fmaxf(sk, m), den = ex2(sk - top) + sum * ex2(m - top);
             sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(m - top) / den;
@@ -686,31 +714,35 @@ attn_kv8_kernel(const AttnKv8Args a) {
 
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
     if (warp < 16 && (any || C == 1)) {
-        const int quad = warp & 3, hh = (warp >> 2 & 1) * 32;
+        const int quad = warp & 3, hh = (warp >> 2 & 1) * W;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const int heads = min(nh - hh, 32), item = C == 1 && a.o_bf16 ? 2 : 4;
+        constexpr int E = W < 16 ? W : 16;
+        const int heads = min(nh - hh, W), item = C == 1 && a.o_bf16 ? 2 : 4;
         // 16 heads at a time and not 32: half the code, which has to be fetched for few rounds of it
 #pragma unroll 1
-        for (int k0 = 0; k0 < heads; k0 += 16) {
-            float f[16];
+        for (int k0 = 0; k0 < heads; k0 += E) {
+            float f[E];
 #pragma unroll
-            for (int k = 0; k < 16; k++) f[k] = sm.f[hh + k0 + k];
+            for (int k = 0; k < E; k++) f[k] = sm.f[hh + k0 + k];
 #pragma unroll 1
             for (int i = warp >> 3; i < NPAIR; i += 2) {
                 const int ch0 = i * 128 + quad * 32;
                 if (ch0 >= a.d) break;
                 const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane); // panels of codes have an order of their own
-                uint32_t v[16];
-                if (any) tmem_ld16(tmem + lanes + i * AK_HEADS + hh + k0, v);
+                uint32_t v[E];
+                if (any) {
+                    ak_ld(tmem + lanes + i * H + hh + k0, v);
+                    ak_ld_wait();
+                }
                 if (C > 1) {
                     float *p = part + (hh + k0) * a.d + ch;
 #pragma unroll
-                    for (int k = 0; k < 16; k++, p += a.d)
+                    for (int k = 0; k < E; k++, p += a.d)
                         if (k0 + k < heads) __stcg(p, __uint_as_float(v[k]));
                 } else {                                 // the output's rows in shared memory, a warp's 32 channels of a head at a time
                     const uint32_t base = smem_u32(smem) + ((hh + k0) * a.d + ch) * item, step = a.d * item;
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
+                    for (int k = 0; k < E; k++) {
                         const uint32_t u = any ? bf16x2_rn(0.f, __uint_as_float(v[k]) * f[k]) : 0u;
                         if (a.o_bf16) asm volatile("st.shared.u16 [%0], %1;" ::"r"(base + k * step), "h"((uint16_t)(u >> 16)));
                         else asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + k * step), "r"(u));
@@ -721,15 +753,15 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     if (C > 1) {
         // the other CTAs of a row must not join what a wait that ran out has left
-        if (tid < AK_HEADS && *s_abort) reinterpret_cast<float2 *>(part + AK_HEADS * a.d)[tid] = make_float2(NAN, NAN);
+        if (tid < H && *s_abort) reinterpret_cast<float2 *>(part + H * a.d)[tid] = make_float2(NAN, NAN);
         __syncwarp();
         cluster_arrive();
         cluster_wait();                                  // the parts of all CTAs are written
         if (!*s_abort) {
             const float *parts = part - (size_t)rank * part_size, *sinks = a.sink ? a.sink + h0 : nullptr;
             void *o = static_cast<uint8_t *>(a.o) + o_at * (a.o_bf16 ? 2 : 4);
-            if (C <= 4) ak_join<4, 2>(C, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
-            else ak_join<1, 8>(C, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            if (C <= 4) ak_join<4, 2>(C, H, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
+            else ak_join<1, 8>(C, H, sm.f, parts, a.d, sinks, o, a.o_bf16, rank, nh);
         }
     } else {
         proxy_fence();
@@ -749,34 +781,52 @@ attn_kv8_kernel(const AttnKv8Args a) {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == AK_MMA)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(K::COLUMNS) : "memory");
 }
 
-// CTAs per query row, and tokens per tile.  `slots`: clusters of 1, 2, 4, 8 and 16 CTAs that the GPU holds at once (148, 74, 33,
-// 15 and 7).  The time in microseconds, fitted to measurements: 9.5 for a CTA's start and end, the join, and 3.15 for a tile of 112
-// tokens, times the turns in which the GPU takes the rows.  Measured, 1 / 2 / 4 / 8 / 16 CTAs per row, * where the rule goes:
-//   1 row of 640 candidates    27.3    22.4     18.2    15.0    14.8*
-//   32 of 640                  29.8    25.1     21.1*   45.8    76.2
-//   48 of 640                  31      25.3*    39      62     107
-//   1 of 8,320                247     134       74      44      30.1*
-//   32 of 8,320               259     140       80.9*  135     151
-//   5 of 128                   13.7    13.5     13.6    13.2*   13.4
-void attn_kv8_shape(int idxw, long long rows, const int (&slots)[5], int *cluster, int *unit, int *ahead) {
+using AkKernel = void (*)(AttnKv8Args);
+// A CTA of 64, 32 or 16 heads.  Its times in microseconds, fitted to measurements: start and end; the join of a row's CTAs; a tile
+// of 112 tokens beside 1.2 for one of none.
+struct AkSize { int heads, smem; AkKernel kernel[2]; double start, join, tile; };
+constexpr int AK_SIZES = 3;
+const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64>, attn_kv8_kernel<true, 64>}, 8.8, 3.8, 1.95},
+                                   {32, Ak<32>::SMEM, {attn_kv8_kernel<false, 32>, attn_kv8_kernel<true, 32>}, 6.8, 3.4, 1.65},
+                                   {16, Ak<16>::SMEM, {attn_kv8_kernel<false, 16>, attn_kv8_kernel<true, 16>}, 5.8, 3.0, 1.5}};
+
+// Heads of a CTA (which of ak_sizes), CTAs per query row and block of heads, tokens per tile.  `slots`: clusters of 1, 2, 4, 8 and
+// 16 CTAs that the GPU holds at once (148, 74, 33, 15 and 7).  Fewer heads per CTA do the work on the candidates' rows once
+// more for every block of heads, but where SMs would have nothing to do every step of a row is shorter; more CTAs per row take
+// fewer tiles each and have a join.  The rule takes the least of: turns in which the GPU takes all clusters, times start, join and
+// tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (over 18 shapes its choice was the fastest
+// in 15, at most 5 % behind in the others):
+//                                64 heads per CTA                    32                                  16
+//   1 row of 640 candidates       27.6  22.7  19.7  15.2  14.8        23.4  19.1  16.8  12.5  12.5        21.5  17.6  15.0  11.3* 11.4
+//   6 of 640                      28.8  23.7  20.4  16.1  15.9        24.0  19.4  17.3  13.0* 24.6        22.0  17.9  15.2  22.1  43.0
+//   32 of 640                     30.2  25.2  21.3* 45.8  76.6        25.9  21.4  33.4  60.1 120.0        23.1  35.3  57.2  95.9
+//   1,024 of 640                 206.7*                              340.6                               621.2
+//   1 of 8,320                   249   135    74.6  44.4  30.0       220   119    65.8  38.5  25.6       208   112    61.8  36.5  23.6*
+//   32 of 8,320                  260   141    80.9* 134   151        231   125   141   195   254         219   233   262   330
+//   5 of 128, 8 heads             12.8  12.8  12.9  12.4  12.6        10.9  11.2  11.5  11.0  11.2        10.0* 10.9  10.9  10.4  10.7
+int attn_kv8_shape(int idxw, int h, int rows, const int (&slots)[AK_SIZES][5], int *cluster, int *unit, int *ahead) {
     double best = 0;
-    *cluster = 1;
-    *unit = 16;
-    for (int i = 0; i < 5; i++) {
-        const int C = 1 << i;
-        if (slots[i] < 1 || (i && rows << i > AK_MOST_PARTS)) continue;
-        const int k = idxw > AK_TILE * C ? (idxw + AK_TILE * C - 1) / (AK_TILE * C) : 1;      // tiles of the CTA with the most
-        const int u = idxw ? ((idxw + C * k - 1) / (C * k) + 15) & ~15 : 16;
-        const double turns = (double)((rows + slots[i] - 1) / slots[i]);
-        const double t = turns * (9.5 + (C > 1 ? 2.5 + 0.05 * C : 0.0) + k * (1.25 + u / 112.0 * 1.9));
-        if (i == 0 || t < best) { best = t; *cluster = C; *unit = u; *ahead = slots[i]; }
+    int which = 0;
+    for (int z = 0; z < AK_SIZES; z++) {
+        const AkSize &size = ak_sizes[z];
+        const long long units = (long long)rows * ceil_div(h, size.heads);
+        for (int i = 0; i < 5; i++) {
+            const int C = 1 << i;
+            if (slots[z][i] < 1 || (i && units << i > AK_MOST_PARTS)) continue;
+            const int k = idxw > AK_TILE * C ? (idxw + AK_TILE * C - 1) / (AK_TILE * C) : 1;  // tiles of the CTA with the most
+            const int u = idxw ? ((idxw + C * k - 1) / (C * k) + 15) & ~15 : 16;
+            const double turns = (double)((units + slots[z][i] - 1) / slots[z][i]);
+            const double t = turns * (size.start + (C > 1 ? size.join + 0.06 * C : 0.0) + k * (1.2 + u / 112.0 * size.tile));
+            if (best == 0 || t < best) { best = t; which = z; *cluster = C; *unit = u; *ahead = slots[z][i]; }
+        }
     }
+    return which;
 }
 
-struct AkDevice { int slots[2][5]; bool ready; };
+struct AkDevice { int slots[2][AK_SIZES][5]; bool ready; };
 // Sets the kernel's attributes on the current device and asks how many clusters of each size it holds, once per device.
 const AkDevice *ak_device() {
     static std::mutex mu;
@@ -786,9 +836,11 @@ const AkDevice *ak_device() {
     std::lock_guard<std::mutex> lock(mu);
     AkDevice &d = at[dev];
     if (d.ready) return &d;
-    for (int tail = 0; tail < 2; tail++) {
-        const void *f = tail ? (const void *)attn_kv8_kernel<true> : (const void *)attn_kv8_kernel<false>;
-        if (ensure_dyn_smem(f, AK_SMEM)) return nullptr;
+    for (int k = 0; k < 2 * AK_SIZES; k++) {
+        const int tail = k & 1;
+        const AkSize &size = ak_sizes[k >> 1];
+        const void *f = (const void *)size.kernel[tail];
+        if (ensure_dyn_smem(f, size.smem)) return nullptr;
         if (cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
         for (int i = 0; i < 5; i++) {
             cudaLaunchConfig_t cfg;
@@ -796,13 +848,13 @@ const AkDevice *ak_device() {
             cudaLaunchAttribute c;
             c.id = cudaLaunchAttributeClusterDimension;
             c.val.clusterDim.x = 1u << i; c.val.clusterDim.y = 1; c.val.clusterDim.z = 1;
-            cfg.gridDim = dim3(1u << i); cfg.blockDim = dim3(AK_THREADS); cfg.dynamicSmemBytes = AK_SMEM;
+            cfg.gridDim = dim3(1u << i); cfg.blockDim = dim3(AK_THREADS); cfg.dynamicSmemBytes = size.smem;
             cfg.attrs = &c; cfg.numAttrs = 1;
             int n = 0;
             if (cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-            d.slots[tail][i] = n;
+            d.slots[tail][k >> 1][i] = n;
         }
-        if (d.slots[tail][0] < 1) { set_error("sparse_attn_kv8: the kernel does not fit the device"); return nullptr; }
+        if (d.slots[tail][k >> 1][0] < 1) { set_error("sparse_attn_kv8: the kernel does not fit the device"); return nullptr; }
     }
     d.ready = true;
     return &d;
@@ -812,10 +864,10 @@ int attn_kv8(AttnKv8Args a, cudaStream_t st) {
     const AkDevice *dev = ak_device();
     a.status = wait_word();
     if (!dev || !a.status) return 1;
-    const unsigned hb = (unsigned)ceil_div(a.h, AK_HEADS);
-    attn_kv8_shape(a.idxw, (long long)a.rows * hb, dev->slots[a.rd != 0], &a.cluster, &a.unit, &a.ahead);
+    const AkSize &size = ak_sizes[attn_kv8_shape(a.idxw, a.h, a.rows, dev->slots[a.rd != 0], &a.cluster, &a.unit, &a.ahead)];
+    const unsigned hb = (unsigned)ceil_div(a.h, size.heads);
     CallScratch scratch(st);
-    if (a.cluster > 1 && scratch.get((size_t)a.rows * hb * a.cluster * (AK_HEADS * a.d + 2 * AK_HEADS) * sizeof(float))) return 1;
+    if (a.cluster > 1 && scratch.get((size_t)a.rows * hb * a.cluster * size.heads * (a.d + 2) * sizeof(float))) return 1;
     a.part = static_cast<float *>(scratch.p);
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
@@ -825,10 +877,10 @@ int attn_kv8(AttnKv8Args a, cudaStream_t st) {
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)a.rows * (unsigned)a.cluster, hb); cfg.blockDim = dim3(AK_THREADS);
-    cfg.dynamicSmemBytes = AK_SMEM; cfg.stream = st;
+    cfg.dynamicSmemBytes = size.smem; cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    APUS_CUDA_OK(a.rd ? cudaLaunchKernelEx(&cfg, attn_kv8_kernel<true>, a) : cudaLaunchKernelEx(&cfg, attn_kv8_kernel<false>, a));
+    APUS_CUDA_OK(cudaLaunchKernelEx(&cfg, size.kernel[a.rd != 0], a));
     APUS_LAUNCHED();
     return 0;
 }

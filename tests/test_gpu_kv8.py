@@ -378,6 +378,27 @@ def test_ends_of_the_numbers():
     assert not out.any()
 
 
+# rows for which a CTA has 16, 32 and 64 heads, with and without others at its row
+@pytest.mark.parametrize("rows", [1, 6, 12, 30, 60, 160])
+@pytest.mark.parametrize("n", [150, 700])
+def test_masks_and_scores_far_apart_for_any_number_of_rows(rows, n):
+    """Rows in turn: scores that rise by hundreds, fall, rise at the end; holes up to the last entry, behind the first, only."""
+    c = Case(17, n=n, holes=0.0, nb=n, na=0, seqs=rows, shared=True)
+    c.scale = 1.0
+    u = np.zeros(512, np.float32)
+    u[100] = 1.0
+    x = rows_flat(np.random.default_rng(9), 1, n, 512) * 0.25
+    x[0, :, 100] = np.linspace(-300, 300, n)
+    c.kv_b = write_rows(bf16_value(bf16_bits(x.astype(np.float32))), 64)
+    c.q = bf16_value(bf16_bits((c.q * 0.02 + u).astype(np.float32)))
+    c.q[:, 1::4] *= -1
+    up = np.arange(n)
+    for r in range(rows):
+        c.idx[r] = [up, up[::-1], np.where(up >= n - 3, up, up // 4), np.where(up == n - 1, up, -1), np.where(up == 0, up, -1), up * 0 - 1][r % 6]
+    got = c.out()
+    c.check(got, [r for r in range(rows) if r < 6 or r >= rows - 6])
+
+
 def test_large_and_small_rows():
     """Scale bytes up to the largest that BF16 holds the values of, and down to the smallest that is written."""
     c = Case(11, n=100, holes=0.0, nb=60, na=0)
