@@ -705,12 +705,15 @@ attn_kv8_kernel(const AttnKv8Args a) {
             sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(m - top) / den;
         }
     }
-    if (warp < AK_MMA) {
+    // A CTA that writes its part to global memory takes every pair of panels as its MMAs end (a CTA of its own uses the panels'
+    // place and waits for all of them); a warp that has not gone through the tiles, because d is small, waits for all too.
+    const bool by_pairs = C > 1 && done;
+    if (warp < AK_MMA && !by_pairs) {
         if (!warp_wait(&sm.o_done, 0u, s_abort)) fail = 56;
-        if (fail) *s_abort = 1;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    __syncthreads();
+    if (fail) *s_abort = 1;
+    if (C == 1) __syncthreads();
 
     const size_t o_at = ((size_t)row * a.h + h0) * a.d;
     if (warp < 16 && (any || C == 1)) {
@@ -729,6 +732,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 const int ch0 = i * 128 + quad * 32;
                 if (ch0 >= a.d) break;
                 const int ch = ch0 + (ch0 < a.d - a.rd ? ak_order(lane) : lane); // panels of codes have an order of their own
+                if (by_pairs && k0 == 0) {
+                    if (!warp_wait(&sm.empty[i], (done - 1) & 1u, s_abort)) fail = 56;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
                 uint32_t v[E];
                 if (any) {
                     ak_ld(tmem + lanes + i * H + hh + k0, v);
@@ -753,6 +760,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
     }
     if (C > 1) {
         // the other CTAs of a row must not join what a wait that ran out has left
+        if (fail) *s_abort = 1;
+        __syncthreads();
         if (tid < H && *s_abort) reinterpret_cast<float2 *>(part + H * a.d)[tid] = make_float2(NAN, NAN);
         __syncwarp();
         cluster_arrive();
