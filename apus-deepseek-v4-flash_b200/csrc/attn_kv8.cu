@@ -268,6 +268,7 @@ struct TileIds {
 template <bool TAIL>
 struct TileRows {
     uint4 v[4][2][2];                                   // panel, row, half
+    uint4 v1[2];                                        // as fetched: the second half of the rotated panel, row
     uint32_t sc[2];
     // `from`: of this lane's bytes in the group's first panel; the first n_codes panels hold codes, the n-th may be rotated
     __device__ __forceinline__ void load(const Kv8Seq &at, const TileIds &ids, int w, int lane, int from, int scales, int n_codes, int n) {
@@ -282,26 +283,23 @@ struct TileRows {
             rec[i] = at.at(id);
             sc[i] = ldg4_if(rec[i] + scales, is[i]);
         }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j < n_codes) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) v[j][i][0] = ldg16_if(rec[i] + from + j * 64, is[i]);
-            } else if (TAIL && j < n) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    v[j][i][0] = ldg16_if(rec[i] + from + j * 64 + sub * 16, is[i]);
-                    v[j][i][1] = ldg16_if(rec[i] + from + j * 64 + sub * 16 + 16, is[i]);
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void convert(int n_codes) {
+        // no branches: every register gets a value, or the loops around this would keep old ones
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (j < n_codes)
 #pragma unroll
-                for (int i = 0; i < 2; i++) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
+            for (int i = 0; i < 2; i++) v[j][i][0] = ldg16_if(rec[i] + from + j * 64 + (TAIL && j >= n_codes ? sub * 16 : 0), is[i] && j < n);
+        if (TAIL)
+#pragma unroll
+            for (int i = 0; i < 2; i++) v1[i] = ldg16_if(rec[i] + from + n_codes * 64 + sub * 16 + 16, is[i] && n_codes < n);
+    }
+    __device__ __forceinline__ void convert(int i2, int n_codes) {       // panels 2 i2 and 2 i2 + 1
+#pragma unroll
+        for (int j = 2 * i2; j < 2 * i2 + 2; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (!TAIL || j < n_codes) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
+                else v[j][i][1] = v1[i];
+            }
     }
     // panels 2 i2 and 2 i2 + 1 of the group's n into shared memory; `to`: where this lane's part of row r0 starts in the group's
     // first panel; the halves of its 16 channels go to x0 and x1
@@ -561,7 +559,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
             cur.load(a, ids, tile, lane);
-            rows.convert(n_codes);                       // before there is room for it, while the tile before is worked on
+            rows.convert(0, n_codes);                    // before there is room for it, while the tile before is worked on
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (2 * i >= n) break;
@@ -569,6 +567,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 if (w * 16 < held) rows.store(to, i, n, n_codes, x0, x1);
                 proxy_fence();
                 mbar_arrive_warp(&sm.full[2 * grp + i], lane);
+                if (i == 0) rows.convert(1, n_codes);    // while the MMAs work on the first ones
             }
             // The next tile's rows, all at once: between the stores above their issue would hold up the second one, and the MMAs
             // that wait for it.
@@ -650,23 +649,17 @@ attn_kv8_kernel(const AttnKv8Args a) {
                     ak_ld_wait();
                 }
                 // all references before the first store: a load behind a store waits for it to issue, one piece after another
-                float4 m[W / 4];
+                uint32_t top = 0, w[W / 2];              // the largest numerator: as BF16 bits they compare like numbers
 #pragma unroll
-                for (int i = 0; i < W / 4; i++) m[i] = mp[i];
-                uint32_t top = 0;                        // the largest numerator: as BF16 bits they compare like numbers
-#pragma unroll
-                for (int c = 0; c < W / 8; c++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int i = 8 * c + 4 * k;
-                        const float4 r = m[2 * c + k];
-                        w[2 * k] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i]), cs, -r.x)), ex2(fmaf(__uint_as_float(s[i + 1]), cs, -r.y)));
-                        w[2 * k + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[i + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[i + 3]), cs, -r.w)));
-                        top = max_u16x2(top, max_u16x2(w[2 * k], w[2 * k + 1]));
-                    }
-                    sts16(prow + ((((hh >> 3) + c) ^ K::p_swizzle(token)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                for (int c = 0; c < W / 4; c++) {
+                    const float4 r = mp[c];
+                    w[2 * c] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[4 * c]), cs, -r.x)), ex2(fmaf(__uint_as_float(s[4 * c + 1]), cs, -r.y)));
+                    w[2 * c + 1] = mask & bf16x2_rn(ex2(fmaf(__uint_as_float(s[4 * c + 2]), cs, -r.z)), ex2(fmaf(__uint_as_float(s[4 * c + 3]), cs, -r.w)));
+                    top = max_u16x2(top, max_u16x2(w[2 * c], w[2 * c + 1]));
                 }
+#pragma unroll
+                for (int c = 0; c < W / 8; c++)
+                    sts16(prow + ((((hh >> 3) + c) ^ K::p_swizzle(token)) << 4), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
                 // a numerator above 2^AK_SLACK: once more with new references
                 if (!soft_any(max(top & 0xffffu, top >> 16) > (127u + AK_SLACK) << 7) || set) break;
             }
