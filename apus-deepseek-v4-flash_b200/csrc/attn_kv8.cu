@@ -68,43 +68,45 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
-// One query row has 64 heads on the same latent rows: 256 operations for every byte of the cache, where this GPU's ratio
-// of tensor rate to memory rate is 253.  So both contractions go to the tensor cores (tcgen05, BF16 operands, f32 sums), a
+// One query row has 64 heads on the same latent rows: 256 operations for every byte of the cache, where this GPU's ratio of
+// tensor rate to memory rate is 253.  So both contractions go to the tensor cores (tcgen05, BF16 operands, f32 sums), a
 // cache row is fetched and dequantised once for all heads, and it serves as key and as value from the same place:
 //
 //   S^T[token, head]   = K[token, ch] Q[head, ch]^T     A = 128 rows as they lie (K-major),  B = the queries
 //   O^T[ch, head]     += V[token, ch]^T P[token, head]   A = the same rows (MN-major),         B = the numerators
 //
 // With tokens, then channels as the 128 rows of an instruction, the heads are its columns (64, 32 or 16 in a CTA:
-// attn_kv8_shape) and no instruction runs half empty.  A group of codes times its power of two is a BF16 value exactly (4 significant bits), so nothing is rounded
-// before the products.  A token is a TMEM lane, so that a thread turns one token's scores into numerators for 32 heads and
-// stores them as one contiguous piece of a row of P.
+// attn_kv8_shape) and no instruction runs half empty.  A group of codes times its power of two is a BF16 value exactly (4
+// significant bits), so nothing is rounded before the products.  A token is a TMEM lane, so that a thread turns one token's
+// scores into numerators for 32 heads and stores them as one contiguous piece of a row of P.
 //
-// The softmax is one pass with a reference per head instead of the running maximum: it is set AK_ABOVE powers of two above the
-// first tile's maximum and stays until a score exceeds it by more than AK_SLACK of them, which in f32 and BF16, floating as both
-// are, costs no precision: numerators of 2^-48 to 2^64 are as good as those around 1, and what is below 2^-126 is less than
-// 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles.  (With the reference at the maximum
-// itself, heads whose scores spread over some 50 powers of two set it anew in three of nineteen tiles: 1,024 rows of 640
-// candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)  Sums of numerators stay in each thread until the end.
+// The softmax is one pass with a reference per head instead of the running maximum: it is set AK_ABOVE powers of two above
+// the first tile's maximum and stays until a score exceeds it by more than AK_SLACK of them, which in f32 and BF16, floating
+// as both are, costs no precision: numerators of 2^-48 to 2^64 are as good as those around 1, and what is below 2^-126 is
+// less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles.  (With the
+// reference at the maximum itself, heads whose scores spread over some 50 powers of two set it anew in three of nineteen
+// tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)  Sums of numerators stay in each
+// thread until the end.
 //
-// A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA
-// writes its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts
-// of its share of the heads in rank order: one launch, the same bits every time.  Through L2, which takes 3,300 cycles
-// to write and 3,200 to 6,800 to read 128 KB per SM; distributed shared memory moved 15 bytes a cycle into an SM, 8,700 cycles.
+// A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA writes
+// its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts of
+// its share of the heads in rank order: one launch, the same bits every time.  Through L2, which takes 3,300 cycles to write
+// and 3,200 to 6,800 to read 128 KB per SM; distributed shared memory moved 15 bytes a cycle into an SM, 8,700 cycles.
 //
-// Warps 0 to 7: softmax, two threads per token, half of the heads each (one thread with all 64: the numerators 500 cycles later,
-// a tile 4 % slower).  Warps 8 to 21: rows, fetched into registers a tile ahead and dequantised into shared memory, the first seven of
-// them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other one dequantises.  Warp 22
-// issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows), Q as 8 panels of the
-// heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight occupies L1, and L1 is what
-// shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and gathered rows arrive at 3.4
-// TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel are the next panel's; what
-// comes of them is masked.)
+// Warps 0 to 7: softmax, two threads per token, half of the heads each (one thread with all 64: the numerators 500 cycles
+// later, a tile 4 % slower).  Warps 8 to 21: rows, fetched into registers a tile ahead and dequantised into shared memory,
+// the first seven of them panels 0 to 3, the others the rest: while one group waits for room to issue its loads, the other
+// one dequantises.  Warp 22 issues the MMAs.  Shared memory: 8 panels of 112 tokens x 64 channels (128-byte swizzled rows),
+// Q as 8 panels of the heads x 64 channels, P.  112 tokens and not the 128 of an instruction, because a load in flight
+// occupies L1, and L1 is what shared memory leaves of 256 KB: with more than 195 KB of shared memory 28 KB are left, and
+// gathered rows arrive at 3.4 TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel
+// are the next panel's; what comes of them is masked.)
 //
-// A tile takes 6,300 cycles with 64 heads (5,700 with 32, 5,400 with 16).  In 4,000 of them shared memory is busy: 60 MMAs read 6 KB each at 128 bytes a cycle, and the rows'
-// 112 KB are written while the MMAs of the tile before, panel pair by panel pair, leave their place.  In the other 2,000 the
-// tensor cores wait for the numerators.  (Two tiles of 64 and 48 tokens in turn, the one's scores under the other's softmax, took
-// 7,300: an instruction of 64 rows takes as long as one of 128.)
+// A tile takes 6,000 cycles with 64 heads (5,300 with 32, 5,200 with 16).  In 4,000 of them shared memory is busy: 60 MMAs
+// read 6 KB each at 128 bytes a cycle, and the rows' 112 KB are written while the MMAs of the tile before, panel pair by
+// panel pair, leave their place.  In the other 2,000 the tensor cores wait for the numerators.  (Two tiles of 64 and 48
+// tokens in turn, the one's scores under the other's softmax, took 7,300 where it was 6,300 so: an instruction of 64 rows
+// takes as long as one of 128.)
 constexpr int AK_TILE = 112, AK_HEADS = 64;             // of the largest CTA
 constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_Q_OFF = 8 * AK_PANEL;
@@ -503,7 +505,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         const uint32_t id_s = ak_idesc(H, false), id_o = ak_idesc(H, true);
         const uint64_t dk = umma_desc_sw128(smem_u32(smem)), dq = umma_desc_sw128(smem_u32(smem + AK_Q_OFF));
         const uint64_t dv = ak_desc_mn(smem_u32(smem), 128), dp = ak_desc_mn(smem_u32(smem + K::P_OFF), K::P_ROW);
-        // The queries of the row that a later CTA on this SM may have, into L2 (1,024 rows of 640 candidates: 209 us without, 206 with)
+        // The queries of the row that a later CTA on this SM may have, into L2 (1,024 rows of 640 candidates: 209.6 us without, 207.0 with)
         if (rank == 0 && lane == 0 && row + (uint32_t)a.ahead < (uint32_t)a.rows) {
             const uint32_t item = a.q_bf16 ? 2u : 4u;
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
@@ -791,24 +793,24 @@ using AkKernel = void (*)(AttnKv8Args);
 // of 112 tokens beside 1.2 for one of none.
 struct AkSize { int heads, smem; AkKernel kernel[2]; double start, join, tile; };
 constexpr int AK_SIZES = 3;
-const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64>, attn_kv8_kernel<true, 64>}, 8.8, 3.8, 1.95},
-                                   {32, Ak<32>::SMEM, {attn_kv8_kernel<false, 32>, attn_kv8_kernel<true, 32>}, 6.8, 3.4, 1.65},
-                                   {16, Ak<16>::SMEM, {attn_kv8_kernel<false, 16>, attn_kv8_kernel<true, 16>}, 5.8, 3.0, 1.5}};
+const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64>, attn_kv8_kernel<true, 64>}, 8.4, 3.9, 1.8},
+                                   {32, Ak<32>::SMEM, {attn_kv8_kernel<false, 32>, attn_kv8_kernel<true, 32>}, 6.2, 3.0, 1.5},
+                                   {16, Ak<16>::SMEM, {attn_kv8_kernel<false, 16>, attn_kv8_kernel<true, 16>}, 5.8, 2.8, 1.5}};
 
 // Heads of a CTA (which of ak_sizes), CTAs per query row and block of heads, tokens per tile.  `slots`: clusters of 1, 2, 4, 8 and
 // 16 CTAs that the GPU holds at once (148, 74, 33, 15 and 7).  Fewer heads per CTA do the work on the candidates' rows once
 // more for every block of heads, but where SMs would have nothing to do every step of a row is shorter; more CTAs per row take
 // fewer tiles each and have a join.  The rule takes the least of: turns in which the GPU takes all clusters, times start, join and
-// tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (over 18 shapes its choice was the fastest
-// in 15, at most 5 % behind in the others):
+// tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (over 18 shapes its choice was within 1 % of
+// the fastest in 17, 5 % behind in one):
 //                                64 heads per CTA                    32                                  16
-//   1 row of 640 candidates       27.6  22.7  19.7  15.2  14.8        23.4  19.1  16.8  12.5  12.5        21.5  17.6  15.0  11.3* 11.4
-//   6 of 640                      28.8  23.7  20.4  16.1  15.9        24.0  19.4  17.3  13.0* 24.6        22.0  17.9  15.2  22.1  43.0
-//   32 of 640                     30.2  25.2  21.3* 45.8  76.6        25.9  21.4  33.4  60.1 120.0        23.1  35.3  57.2  95.9
-//   1,024 of 640                 206.7*                              340.6                               621.2
-//   1 of 8,320                   249   135    74.6  44.4  30.0       220   119    65.8  38.5  25.6       208   112    61.8  36.5  23.6*
-//   32 of 8,320                  260   141    80.9* 134   151        231   125   141   195   254         219   233   262   330
-//   5 of 128, 8 heads             12.8  12.8  12.9  12.4  12.6        10.9  11.2  11.5  11.0  11.2        10.0* 10.9  10.9  10.4  10.7
+//   1 row of 640 candidates       26.8  21.3  18.7  14.3  14.0        22.8  17.9  15.8  11.6  11.7        21.6  16.9  14.4  10.8* 11.0
+//   6 of 640                      27.9  22.4  19.7  15.2  15.1        23.2  18.1  16.2  12.0* 22.7        21.9  17.1  14.7  20.8  40.9
+//   32 of 640                     29.2  23.9  20.1  43.3  72.7        24.1  19.1* 31.0  55.1 111.1        22.5  33.6  54.7  90.3
+//   1,024 of 640                 200.7*                              332.3                               619.4
+//   1 of 8,320                   241   130    71.4  42.3  28.4       214   115    63.6  37.0  24.3       208   111    61.0  35.4  22.9*
+//   32 of 8,320                  247   135    77.2* 128   143        225   122   137   188   242         214   227   255   320
+//   5 of 128, 8 heads             12.7  12.6  12.6  12.2  12.4        10.9  11.1  11.3  10.8  11.1        10.2* 10.8  10.7  10.3  10.5
 int attn_kv8_shape(int idxw, int h, int rows, const int (&slots)[AK_SIZES][5], int *cluster, int *unit, int *ahead) {
     double best = 0;
     int which = 0;
