@@ -596,7 +596,9 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const uint32_t mask = valid ? ~0u : 0u;      // not a choice: the compiler would branch around every numerator
             tile += C;
             cur.load(a, ids, tile, lane);
-            if (!warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
+            // One warp polls: the issue slots are the row warps'.  Behind this the numerators of the tile before have been added up.
+            if (warp == 0 && !warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
+            soft_sync();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (bool set = done == 0;; set = true) {
                 uint32_t s[W];
@@ -677,7 +679,6 @@ attn_kv8_kernel(const AttnKv8Args a) {
                 l[4] += __uint_as_float(w.z << 16); l[5] += __uint_as_float(w.z & 0xffff0000u);
                 l[6] += __uint_as_float(w.w << 16); l[7] += __uint_as_float(w.w & 0xffff0000u);
             }
-            soft_sync();                                 // before the next tile's numerators take their place
             if (fail) *s_abort = 1;
             done++;
             settle();
