@@ -808,7 +808,7 @@ const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64
 //   1 row of 640 candidates       26.8  21.3  18.7  14.3  14.0        22.8  17.9  15.8  11.6  11.7        21.6  16.9  14.4  10.8* 11.0
 //   6 of 640                      27.9  22.4  19.7  15.2  15.1        23.2  18.1  16.2  12.0* 22.7        21.9  17.1  14.7  20.8  40.9
 //   32 of 640                     29.2  23.9  20.1  43.3  72.7        24.1  19.1* 31.0  55.1 111.1        22.5  33.6  54.7  90.3
-//   1,024 of 640                 200.7*                              332.3                               619.4
+//   1,024 of 640                 199.1*                              332.3                               619.4
 //   1 of 8,320                   241   130    71.4  42.3  28.4       214   115    63.6  37.0  24.3       208   111    61.0  35.4  22.9*
 //   32 of 8,320                  247   135    77.2* 128   143        225   122   137   188   242         214   227   255   320
 //   5 of 128, 8 heads             12.7  12.6  12.6  12.2  12.4        10.9  11.1  11.3  10.8  11.1        10.2* 10.8  10.7  10.3  10.5
