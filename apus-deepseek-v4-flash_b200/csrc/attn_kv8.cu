@@ -807,14 +807,15 @@ const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64
 // fewer tiles each and have a join.  The rule takes the least of: turns in which the GPU takes all clusters, times start, join and
 // tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (over 18 shapes its choice was within 1 % of
 // the fastest in 17, 5 % behind in one):
-//                                64 heads per CTA                    32                                  16
-//   1 row of 640 candidates       26.8  21.3  18.7  14.3  14.0        22.8  17.9  15.8  11.6  11.7        21.6  16.9  14.4  10.8* 11.0
-//   6 of 640                      27.9  22.4  19.7  15.2  15.1        23.2  18.1  16.2  12.0* 22.7        21.9  17.1  14.7  20.8  40.9
-//   32 of 640                     29.2  23.9  20.1  43.3  72.7        24.1  19.1* 31.0  55.1 111.1        22.5  33.6  54.7  90.3
-//   1,024 of 640                 199.1*                              332.3                               619.4
-//   1 of 8,320                   241   130    71.4  42.3  28.4       214   115    63.6  37.0  24.3       208   111    61.0  35.4  22.9*
-//   32 of 8,320                  247   135    77.2* 128   143        225   122   137   188   242         214   227   255   320
-//   5 of 128, 8 heads             12.7  12.6  12.6  12.2  12.4        10.9  11.1  11.3  10.8  11.1        10.2* 10.8  10.7  10.3  10.5
+//                              64 heads per CTA                    32                                  16
+//   1 row of 640 candidates   26.5   21.4   18.9   14.5   14.2    22.8   17.9   15.0   11.7   11.9    21.6   16.8   13.5   10.9*  11.3
+//   6 of 640                  27.6   22.4   19.8   15.4   15.1    23.3   18.1   15.4   12.0*  23.1    21.9   17.0   13.7   21.1   42.1
+//   16 of 640                 28.9   23.8   19.9   29.3   42.9    24.0   19.1   15.6*  33.2   56.0    22.4   17.7   26.1   51.1    104
+//   32 of 640                 29.0   23.9   20.3   43.6   73.2    24.1   19.3*  29.3   55.0    113    22.5   33.5   51.0   91.6
+//   1,024 of 640             199.2*                                332                                 621
+//   1 of 8,320                 238    129   71.4   42.3   28.4     214    115   62.5   36.8   24.2     208    111   60.1   35.6   23.1*
+//   32 of 8,320                246    136   77.1*   128    143     225    121    135    188    242     214    227    251    321
+//   5 of 128, 8 heads         12.6   12.6   12.7   12.3   12.5    10.8   11.1   10.7   11.0   11.2    10.0*  10.7   10.1   10.5   10.8
 int attn_kv8_shape(int idxw, int h, int rows, const int (&slots)[AK_SIZES][5], int *cluster, int *unit, int *ahead) {
     double best = 0;
     int which = 0;
