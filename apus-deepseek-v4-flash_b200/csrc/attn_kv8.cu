@@ -83,10 +83,11 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // The softmax is one pass with a reference per head instead of the running maximum: it is set AK_ABOVE powers of two above
 // the first tile's maximum and stays until a score exceeds it by more than AK_SLACK of them, which in f32 and BF16, floating
 // as both are, costs no precision: numerators of 2^-48 to 2^64 are as good as those around 1, and what is below 2^-126 is
-// less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles.  (With the
-// reference at the maximum itself, heads whose scores spread over some 50 powers of two set it anew in three of nineteen
-// tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)  Sums of numerators stay in each
-// thread until the end.
+// less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles, by a factor of
+// down to 2^-190 and beyond, which f32 does not hold: numerators of 2^64 before are 2^-14 of the new largest one at a factor of
+// 2^-126, so it is applied as two.  (With the reference at the maximum itself, heads whose scores spread over some 50 powers
+// of two set it anew in three of nineteen tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)
+// Sums of numerators stay in each thread until the end.
 //
 // A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA writes
 // its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts of
@@ -169,6 +170,11 @@ __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float r;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
@@ -331,6 +337,11 @@ struct TileRows {
     }
 };
 
+// What a reference and the sum of the numerators relative to it add up to, in powers of two: parts and the sink are weighed
+// against the largest of these and not against the largest reference, which may be far above all its scores.  So a factor that is
+// zero, 2^-126 or less, makes weights zero that are below 2^(AK_SLACK - 126).
+__device__ __forceinline__ float ak_weight(float2 v) { return v.x + lg2(v.y); }
+
 // The parts of a row's C CTAs, joined for this CTA's share of the heads: U times 4 channels of a head and R of the parts at a
 // time, four or eight loads in flight
 template <int U, int R>
@@ -347,7 +358,7 @@ __device__ __forceinline__ void ak_join(int C, int H, float *w, const float *par
             v = __ldcg(reinterpret_cast<const float2 *>(parts + r * part_size + H * d) + lo + hd);
             if (sink) sk = sink[lo + hd] * LOG2E;
         }
-        float top = fmaxf(v.x, sk);
+        float top = fmaxf(fmaxf(ak_weight(v), sk), AK_NONE);
         for (int m = 1; m < C; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
         float den = v.y * ex2(v.x - top);
         for (int m = 1; m < C; m <<= 1) den += __shfl_xor_sync(0xffffffffu, den, m);
@@ -625,13 +636,13 @@ attn_kv8_kernel(const AttnKv8Args a) {
                         const float old = sm.m[tid];
                         const float now = fmaxf(fmaxf(fmaxf(sm.part[0][tid], sm.part[1][tid]), fmaxf(sm.part[2][tid], sm.part[3][tid])) + AK_ABOVE, old);
                         sm.m[tid] = now;
-                        sm.f[tid] = ex2(old - now);
+                        sm.f[tid] = ex2(0.5f * (old - now));     // its square is the factor, which may be below 2^-126
                     }
                     soft_sync();
                     if (done) {
                         const float4 *f = reinterpret_cast<const float4 *>(sm.f + hh);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) l[i] *= sm.f[8 * lh + i];
+                        for (int i = 0; i < 8; i++) { const float g = sm.f[8 * lh + i]; l[i] = l[i] * g * g; }
 #pragma unroll 1
                         for (int i = 0; i < NPAIR; i++) {
                             const uint32_t o = tmem + lanes + i * H + hh;
@@ -640,10 +651,10 @@ attn_kv8_kernel(const AttnKv8Args a) {
 #pragma unroll
                             for (int k = 0; k < W / 4; k++) {
                                 const float4 g = f[k];
-                                s[4 * k] = __float_as_uint(__uint_as_float(s[4 * k]) * g.x);
-                                s[4 * k + 1] = __float_as_uint(__uint_as_float(s[4 * k + 1]) * g.y);
-                                s[4 * k + 2] = __float_as_uint(__uint_as_float(s[4 * k + 2]) * g.z);
-                                s[4 * k + 3] = __float_as_uint(__uint_as_float(s[4 * k + 3]) * g.w);
+                                s[4 * k] = __float_as_uint(__uint_as_float(s[4 * k]) * g.x * g.x);
+                                s[4 * k + 1] = __float_as_uint(__uint_as_float(s[4 * k + 1]) * g.y * g.y);
+                                s[4 * k + 2] = __float_as_uint(__uint_as_float(s[4 * k + 2]) * g.z * g.z);
+                                s[4 * k + 3] = __float_as_uint(__uint_as_float(s[4 * k + 3]) * g.w * g.w);
                             }
                             ak_st(o, s);
                         }
@@ -697,7 +708,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const float m = sm.m[tid];
             if (C > 1) reinterpret_cast<float2 *>(part + H * a.d)[tid] = make_float2(m, sum);
             // the only CTA of its row: what its part is multiplied by, while the last MMAs run
-            const float sk = sink * LOG2E, top = fmaxf(sk, m), den = ex2(sk - top) + sum * ex2(m - top);
+            const float sk = sink * LOG2E, top = fmaxf(fmaxf(ak_weight(make_float2(m, sum)), sk), AK_NONE), den = ex2(sk - top) + sum * ex2(m - top);
             sm.f[tid] = sk == INFINITY || den == 0.f ? 0.f : ex2(m - top) / den;
         }
     }

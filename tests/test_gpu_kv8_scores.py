@@ -1,0 +1,64 @@
+"""Attention over 8-bit caches where scores lie far apart: what a softmax in one pass may drop, and what it must not."""
+import numpy as np
+import pytest
+
+from _gpu import lib, ok                       # noqa: F401
+from _kv8 import attend, bf16_bits, bf16_value, read_rows, tolerance, write_rows
+from test_gpu_kv8 import Case, rows_flat
+
+pytestmark = pytest.mark.gpu
+
+LN2 = float(np.log(2.0))
+
+
+def levels(n, rows, place, level, value=None):
+    """`rows` query rows over one cache whose record i has a score of place-th level[i] powers of two for every head (and a
+    little noise); `value`: rows [records, 512] or random ones."""
+    k = len(level)
+    c = Case(71, n=n, seqs=rows, shared=True, na=0, nb=k, holes=0.0)
+    x = rows_flat(np.random.default_rng(9), 1, k, 512) if value is None else value[None].astype(np.float32)
+    x[0, :, 500] = level
+    c.kv_b = write_rows(bf16_value(bf16_bits(x)), 64)
+    c.q *= np.float32(2.0 ** -8)
+    c.q[:, :, :64] = 0
+    c.q[:, :, 448:] = 0
+    c.q[:, :, 500] = 1
+    c.scale = LN2
+    c.idx[:] = place
+    return c
+
+
+def check(c, got, some):
+    """Case.check, and beside its tolerance what the one pass may drop.  A numerator is dropped below 2^-126, where the reference is
+    48 powers of two above the largest score: a weight below 2^-78.  A part of a row, whose numerators are at most 2^64, is dropped
+    where its factor is below 2^-126: weights below 2^-62, of which 2^-61 is a bound with all roundings."""
+    val = read_rows(c.kv_b[0], c.d, c.rd)
+    for r in some:
+        o, wv, es = attend(c.q[r], val[c.idx[r]], np.ones(c.n, bool), c.scale, c.sink)
+        off = np.abs(got[r] - o) / (tolerance(o, wv, es) + 2.0 ** -61 * np.abs(val[c.idx[r]]).sum(0))
+        assert off.max() <= 1, (r, off.max())
+
+
+# Most candidates weigh 2^-15 of the last one, hundreds or thousands of times, so that they count; they come where the
+# running reference has not moved for long, and the last one moves it.  CTAs that have seen the first ones, all and the
+# last one meet in a join.
+@pytest.mark.parametrize("most", [15.5, 33.0, 47.5, 63.0, 79.5, 95.5, 111.5, 124.0])
+@pytest.mark.parametrize("n,rows,lead", [(640, 1, 80), (640, 1, 450), (640, 160, 112), (640, 1024, 112), (8320, 1, 100), (8320, 1, 1800), (8320, 32, 450)])
+def test_many_candidates_just_below_a_late_maximum(n, rows, lead, most):
+    level = np.concatenate((np.zeros(16), np.full(16, most), [most + 15]))
+    at = np.arange(n)
+    c = levels(n, rows, np.where(at < lead, at % 16, np.where(at < n - 1, 16 + at % 16, 32)), level)
+    x = rows_flat(np.random.default_rng(9), 33, 512)
+    x[16:32, :64], x[32, :64], x[:, 500] = 1.0, 0.0, level
+    c.kv_b = write_rows(x[None], 64)
+    check(c, c.out(), sorted({0, rows - 1}))
+
+
+# A sink above every score, where the scores have risen far above the first reference or stayed far below it.
+@pytest.mark.parametrize("rise,sink", [(0.0, 10.0), (0.0, 50.0), (0.0, -40.0), (60.0, 100.0), (111.0, 121.0), (111.0, 160.0), (111.0, 60.0)])
+@pytest.mark.parametrize("n,rows", [(640, 1), (640, 160), (8320, 2)])
+def test_sinks_far_from_the_reference(n, rows, rise, sink):
+    at = np.arange(n)
+    c = levels(n, rows, np.where(at < n - 30, at % 16, 16 + at % 16), np.concatenate((np.zeros(16), np.full(16, rise))))
+    c.sink[:] = sink * LN2
+    check(c, c.out(), sorted({0, rows - 1}))
