@@ -87,7 +87,9 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // down to 2^-190 and beyond, which f32 does not hold: numerators of 2^64 before are 2^-14 of the new largest one at a factor of
 // 2^-126, so it is applied as two.  (With the reference at the maximum itself, heads whose scores spread over some 50 powers
 // of two set it anew in three of nineteen tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)
-// Sums of numerators stay in each thread until the end.
+// Where a row has values of 2^32 or more, numerators of 2^64 would take the sums out of f32: from there on references are set
+// so that no numerator is above 1, as in a softmax with the maximum at hand.  Sums of numerators stay in each thread until the
+// end.
 //
 // A row's candidates are cut into tiles of at most 112, dealt in turn to the CTAs of a cluster.  At the end every CTA writes
 // its part of O^T, its references and its sums to scratch, meets the others in a cluster barrier and adds up the parts of
@@ -112,7 +114,7 @@ constexpr int AK_TILE = 112, AK_HEADS = 64;             // of the largest CTA
 constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_Q_OFF = 8 * AK_PANEL;
 constexpr int AK_MOST_PARTS = 1024;                     // 135 MB of scratch
-constexpr uint32_t AK_SLACK = 64;                       // as values of rows go up to 2^16, the f32 sums hold 2^40 such products
+constexpr uint32_t AK_SLACK = 64;                       // 2^30 products of such a numerator and a value of up to 2^32 stay in f32
 constexpr float AK_ABOVE = 48.f, AK_NONE = -1.7e38f, LOG2E = 1.4426950408889634f;
 
 struct AkMisc {
@@ -121,7 +123,7 @@ struct AkMisc {
     alignas(16) float part[AK_SOFT][AK_HEADS];
     uint64_t full[4], empty[4], q_full, s_full, p_ready, o_done;
     uint32_t tmem;
-    int abort;
+    int abort, large;                                   // large: a row with values of 2^32 or more has been fetched
 };
 // What depends on the heads of a CTA.
 template <int H>
@@ -181,6 +183,13 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+// Squares of eight BF16 values added to two sums.  Rounding keeps order, so a sum is not below any of its squares: 2^64 or more
+// (or NaN) where a value is 2^32 or more.  One instruction for two values, where magnitudes and their maximum take two.
+__device__ __forceinline__ uint32_t squares_bf16x2(uint32_t s, const uint4 &v) {
+    asm("fma.rn.bf16x2 %0, %1, %1, %0;\n\tfma.rn.bf16x2 %0, %2, %2, %0;\n\tfma.rn.bf16x2 %0, %3, %3, %0;\n\tfma.rn.bf16x2 %0, %4, %4, %0;"
+        : "+r"(s) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+    return s;
 }
 __device__ __forceinline__ void ak_ld(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
 __device__ __forceinline__ void ak_ld(uint32_t taddr, uint32_t (&v)[16]) {
@@ -300,18 +309,26 @@ struct TileRows {
 #pragma unroll
             for (int i = 0; i < 2; i++) v1[i] = ldg16_if(rec[i] + from + n_codes * 64 + sub * 16 + 16, is[i] && n_codes < n);
     }
-    __device__ __forceinline__ void convert(int i2, int n_codes) {       // panels 2 i2 and 2 i2 + 1
+    __device__ __forceinline__ void convert(int i2, int n_codes, volatile int *large) {  // panels 2 i2 and 2 i2 + 1
 #pragma unroll
-        for (int j = 2 * i2; j < 2 * i2 + 2; j++)
+        for (int j = 2 * i2; j < 2 * i2 + 2; j++) {
+            if (!TAIL || j < n_codes) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                if (!TAIL || j < n_codes) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
-                else v[j][i][1] = v1[i];
+                for (int i = 0; i < 2; i++) dequant16(v[j][i][0], sc[i] >> 8 * j & 0xffu, v[j][i][0], v[j][i][1]);
+            } else {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    v[j][i][1] = v1[i];
+                    m = squares_bf16x2(squares_bf16x2(m, v[j][i][0]), v[j][i][1]);
+                }
+                if (max(m & 0xffffu, m >> 16) >= (127u + 64u) << 7) *large = 1;
             }
+        }
     }
     // panels 2 i2 and 2 i2 + 1 of the group's n into shared memory; `to`: where this lane's part of row r0 starts in the group's
     // first panel; the halves of its 16 channels go to x0 and x1
-    __device__ __forceinline__ void store(uint8_t *to, int i2, int n, int n_codes, int x0, int x1) const {
+    __device__ __forceinline__ void store(uint8_t *to, int i2, int n, int n_codes, int x0, int x1, volatile int *large) const {
 #pragma unroll
         for (int j = 2 * i2; j < 2 * i2 + 2; j++)
             if (j < n)
@@ -323,6 +340,7 @@ struct TileRows {
         // the part of a scale above byte 134, on what has been stored (255: NaN)
         const uint32_t top = max_u16x2(max_u16x2(sc[0] & 0x00ff00ffu, sc[0] >> 8 & 0x00ff00ffu), max_u16x2(sc[1] & 0x00ff00ffu, sc[1] >> 8 & 0x00ff00ffu));
         if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > 134u)) {
+            if (max(top & 0xffffu, top >> 16) > 149u) *large = 1;        // a code of up to 2^9 times 2^23
 #pragma unroll 1
             for (int k = 0; k < 32; k++) {
                 const int j = 2 * i2 + (k >> 4), i = k >> 3 & 1;
@@ -415,7 +433,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
     constexpr int W = K::W;
     extern __shared__ __align__(1024) uint8_t smem[];
     AkMisc &sm = *reinterpret_cast<AkMisc *>(smem + K::MISC_OFF);
-    volatile int *s_abort = &sm.abort;
+    volatile int *s_abort = &sm.abort, *s_large = &sm.large;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, C = a.cluster;
     const int rank = (int)(blockIdx.x % (unsigned)C), h0 = (int)blockIdx.y * H, nh = min(H, a.h - h0);
     const uint32_t row = blockIdx.x / (unsigned)C, seq = row / (uint32_t)a.rows_per_seq;
@@ -434,6 +452,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         mbar_init(&sm.s_full, 1);
         mbar_init(&sm.p_ready, AK_SOFT);
         mbar_init(&sm.o_done, 1);
+        *s_large = 0;
         *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -572,15 +591,15 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
             cur.load(a, ids, tile, lane);
-            rows.convert(0, n_codes);                    // before there is room for it, while the tile before is worked on
+            rows.convert(0, n_codes, s_large);                    // before there is room for it, while the tile before is worked on
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (2 * i >= n) break;
                 if (!warp_wait(&sm.empty[2 * grp + i], (done & 1u) ^ 1u, s_abort)) fail = 54;
-                if (w * 16 < held) rows.store(to, i, n, n_codes, x0, x1);
+                if (w * 16 < held) rows.store(to, i, n, n_codes, x0, x1, s_large);
                 proxy_fence();
                 mbar_arrive_warp(&sm.full[2 * grp + i], lane);
-                if (i == 0) rows.convert(1, n_codes);    // while the MMAs work on the first ones
+                if (i == 0) rows.convert(1, n_codes, s_large);   // while the MMAs work on the first ones
             }
             // The next tile's rows, all at once: between the stores above their issue would hold up the second one, and the MMAs
             // that wait for it.
@@ -607,10 +626,16 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const uint32_t mask = valid ? ~0u : 0u;      // not a choice: the compiler would branch around every numerator
             tile += C;
             cur.load(a, ids, tile, lane);
-            // One warp polls: the issue slots are the row warps'.  Behind this the numerators of the tile before have been added up.
-            if (warp == 0 && !warp_wait(&sm.s_full, done & 1u, s_abort)) fail = 55;
+            // One warp polls: the issue slots are the row warps'.  It waits for the rows, too, for what they say about their values.
+            // Behind this the numerators of the tile before have been added up.
+            if (warp == 0) {
+#pragma unroll 1
+                for (int i = 0; i <= NPAIR; i++)
+                    if (!warp_wait(i < NPAIR ? &sm.full[i] : &sm.s_full, done & 1u, s_abort)) fail = 55;
+            }
             soft_sync();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t most = (127u + (*s_large ? 0u : AK_SLACK)) << 7;
             for (bool set = done == 0;; set = true) {
                 uint32_t s[W];
                 ak_ld(tmem_s + lanes + hh, s);
@@ -675,8 +700,8 @@ attn_kv8_kernel(const AttnKv8Args a) {
 #pragma unroll
                 for (int c = 0; c < W / 8; c++)
                     sts16(prow + ((((hh >> 3) + c) ^ K::p_swizzle(token)) << 4), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
-                // a numerator above 2^AK_SLACK: once more with new references
-                if (!soft_any(max(top & 0xffffu, top >> 16) > (127u + AK_SLACK) << 7) || set) break;
+                // a numerator above 2^AK_SLACK, or above 1 where values are large: once more with new references
+                if (!soft_any(max(top & 0xffffu, top >> 16) > most) || set) break;
             }
             proxy_fence();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -550,8 +550,8 @@ int apus_cuda_kv8_read_dev(const uint8_t *cache, int d, int rd, int64_t cap, int
  * same call gives the same bits; how many SMs share a row, and with it the order of the sums,
  * follows from rows, h and idxw.  Where several do, the call uses a scratch buffer of the library
  * that belongs to its stream (at most 135 MB), one that is being recorded gets memory that its
- * graph owns.  Weights below 2^-62 and values of rows below 2^-78 may count as zero.  h: up to
- * 1,024; idxw: up to 2^30; na + nb < 2^31. */
+ * graph owns.  Weights below 2^-62 and values of rows below 2^-78 may count as zero; there is no
+ * upper limit but f32's on the weighted sums.  h: up to 1,024; idxw: up to 2^30; na + nb < 2^31. */
 int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const float *sink, int h, int d,
                                   int rd, const int32_t *idxs, int idxw, int rows,
                                   int rows_per_seq, float scale, const uint8_t *kv_a, int64_t na,

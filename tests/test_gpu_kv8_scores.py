@@ -12,17 +12,18 @@ LN2 = float(np.log(2.0))
 
 
 def levels(n, rows, place, level, value=None):
-    """`rows` query rows over one cache whose record i has a score of place-th level[i] powers of two for every head (and a
-    little noise); `value`: rows [records, 512] or random ones."""
+    """`rows` query rows over one cache, whose record i has a score of level[i] powers of two for every head (and a little
+    noise); candidate j is record place[j].  `value`: the records' rows [len(level), d], or random ones of 512."""
     k = len(level)
-    c = Case(71, n=n, seqs=rows, shared=True, na=0, nb=k, holes=0.0)
-    x = rows_flat(np.random.default_rng(9), 1, k, 512) if value is None else value[None].astype(np.float32)
-    x[0, :, 500] = level
-    c.kv_b = write_rows(bf16_value(bf16_bits(x)), 64)
+    x = rows_flat(np.random.default_rng(9), k, 512) if value is None else value.astype(np.float32)
+    d = x.shape[1]
+    c = Case(71, n=n, d=d, seqs=rows, shared=True, na=0, nb=k, holes=0.0)
+    x[:, d - 12] = level
+    c.kv_b = write_rows(bf16_value(bf16_bits(x)), 64)[None]
     c.q *= np.float32(2.0 ** -8)
     c.q[:, :, :64] = 0
-    c.q[:, :, 448:] = 0
-    c.q[:, :, 500] = 1
+    c.q[:, :, d - 64:] = 0
+    c.q[:, :, d - 12] = 1
     c.scale = LN2
     c.idx[:] = place
     return c
@@ -62,3 +63,19 @@ def test_sinks_far_from_the_reference(n, rows, rise, sink):
     c = levels(n, rows, np.where(at < n - 30, at % 16, 16 + at % 16), np.concatenate((np.zeros(16), np.full(16, rise))))
     c.sink[:] = sink * LN2
     check(c, c.out(), sorted({0, rows - 1}))
+
+
+# Rows of any size that a record holds, in the codes (a scale byte far above the others') or in the rotated channels, behind
+# scores that let the numerators grow: where the sums of the definition are numbers, so are these.
+@pytest.mark.parametrize("rise", [0.0, 30.0, 47.5, 49.0, 63.0, 100.0, 111.5, 140.0])
+@pytest.mark.parametrize("power,late", [(31, 300), (33, 300), (60, 1), (80, 1), (115, 300), (120, 1)])
+@pytest.mark.parametrize("n,rows,d,channel", [(640, 1, 512, 3), (640, 160, 512, 3), (640, 160, 512, 450), (8320, 2, 512, 450), (640, 160, 192, 3), (640, 160, 192, 130)])
+def test_large_values_behind_scores_that_rise(n, rows, d, channel, rise, power, late):
+    level = np.concatenate((np.zeros(16), np.full(16, rise)))
+    x = rows_flat(np.random.default_rng(9), 32, d)
+    x[16:, channel] = -1.5 * 2.0 ** power
+    at = np.arange(n)
+    c = levels(n, rows, np.where(at < n - late, at % 16, 16 + at % 16), level, x)
+    got = c.out()
+    assert np.isfinite(got).all()
+    check(c, got, sorted({0, rows - 1}))
