@@ -79,3 +79,24 @@ def test_large_values_behind_scores_that_rise(n, rows, d, channel, rise, power, 
     got = c.out()
     assert np.isfinite(got).all()
     check(c, got, sorted({0, rows - 1}))
+
+
+# Every score is exact and thousands away from the next one, up to the end of f32, so that the result is the row of the largest
+# one, or nothing beside a sink far above.
+@pytest.mark.parametrize("n,rows", [(1, 1), (120, 1), (700, 1), (700, 160)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [20, 24, 31, 60, 90, 118])
+def test_scores_up_to_the_largest_numbers(power, sign, n, rows):
+    c = Case(41, n=n, holes=0.0, na=0, nb=128, seqs=rows, shared=True)
+    x = rows_flat(np.random.default_rng(9), 128, 512)
+    x[:, 500] = 1 + np.arange(128) / 128.0
+    c.kv_b = write_rows(x, 64)[None]
+    c.q[:] = 0
+    c.q[:, :, 500] = 2.0 ** (np.arange(64) % 8)
+    c.scale = sign * 2.0 ** power
+    c.idx[:] = np.random.default_rng(5).integers(0, 128, (rows, n))
+    best = c.idx.max(1) if sign > 0 else c.idx.min(1)
+    want = np.broadcast_to(read_rows(c.kv_b[0, best], 512, 64)[:, None], (rows, 64, 512))
+    assert np.array_equal(c.out(), want if sign > 0 else np.zeros_like(want))
+    c.sink = None
+    assert np.array_equal(c.out(), want)
