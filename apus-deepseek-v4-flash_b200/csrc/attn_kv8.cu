@@ -951,7 +951,7 @@ extern "C" int apus_cuda_sparse_attn_kv8_dev(const void *q, int q_bf16, const fl
     APUS_REQUIRE(h > 0 && h <= 1024, "sparse_attn_kv8: h=%d must be 1 to 1024", h);
     APUS_REQUIRE(rows >= 0 && idxw >= 0 && idxw <= 1 << 30, "sparse_attn_kv8: %d rows of %d ids", rows, idxw);
     APUS_REQUIRE(rows_per_seq > 0 && rows % rows_per_seq == 0, "sparse_attn_kv8: %d rows are not sequences of %d", rows, rows_per_seq);
-    APUS_REQUIRE(na >= 0 && nb >= 0 && na + nb <= INT32_MAX, "sparse_attn_kv8: na=%lld, nb=%lld", (long long)na, (long long)nb);
+    APUS_REQUIRE(na >= 0 && nb >= 0 && na <= INT32_MAX && nb <= INT32_MAX - na, "sparse_attn_kv8: na=%lld, nb=%lld", (long long)na, (long long)nb);
     APUS_REQUIRE(kv_a_stride >= 0 && kv_b_stride >= 0, "sparse_attn_kv8: negative stride");
     APUS_REQUIRE((na == 0 || kv_a) && (nb == 0 || kv_b), "sparse_attn_kv8: no cache");
     APUS_REQUIRE(aligned16(kv_a) && aligned16(kv_b), "sparse_attn_kv8: the caches must start on a 16-byte boundary");

@@ -60,3 +60,8 @@ def test_nothing_to_do_needs_no_device():
                              ("apus_cuda_kv8_write_dev", WRITE, dict(cap=0, cache=None)), ("apus_cuda_kv8_read_dev", READ, dict(s=0)),
                              ("apus_cuda_sparse_attn_kv8_dev", ATTN, dict(rows=0, per=1, q=None, o=None))):
         assert getattr(L, fn)(*dict(base, **change).values()) == 0, L.apus_cuda_last_error()
+
+
+@pytest.mark.parametrize("na,nb", [((1 << 63) - 1, (1 << 63) - 1), (1 << 62, 1 << 62), ((1 << 62) + 5, (1 << 63) - (1 << 62)), (1 << 31, 0), (1, (1 << 31) - 1)])
+def test_cache_sizes_whose_sum_leaves_its_type(na, nb):
+    refused("apus_cuda_sparse_attn_kv8_dev", ATTN, dict(na=na, nb=nb), "na=")
