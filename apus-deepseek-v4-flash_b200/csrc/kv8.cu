@@ -62,7 +62,7 @@ kv8_write_kernel(const void *x, int d, int rd, uint32_t rows, uint32_t s, const 
     const uint32_t b = row / s;
     const int t = (int)(row - b * s), n = counts ? min(max(counts[b], 0), (int)s) : (int)s;
     long long at = (long long)((unsigned long long)pos[b] + t);          // beyond the last of all numbers: a negative one
-    if (t >= n || at < 0 || (ring ? (long long)n - t > cap : at >= cap)) return;
+    if (t >= n || at < 0 || (ring ? (long long)n - t > cap && at <= INT64_MAX - cap : at >= cap)) return;     // in a ring: unless row t + cap has the place
     if (at >= cap) at = (uint64_t)(at | cap) >> 32 ? at % cap : (uint32_t)at % (uint32_t)cap;
     uint8_t *rec = cache + (size_t)(b * stride + at) * kv8_row_bytes(d, rd);
     uint32_t sc[KV8_STEPS];                                      // the row's scale bytes, in every lane

@@ -1,0 +1,18 @@
+"""The cache of latent rows held in 8 bits at further ends: positions at the last number, other strides, types and row shapes."""
+import numpy as np
+import pytest
+
+from _kv8 import write_rows
+from test_gpu_kv8 import rows, same, write
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("back,cap,s", [(3, 2, 6), (3, 1, 6), (1, 4, 9), (5, 5, 20), (6, 4, 6)])
+def test_a_ring_at_the_end_of_the_numbers_keeps_the_last_row_that_has_an_entry(back, cap, s):
+    x = rows(np.random.default_rng(s), 1, s, 128)
+    got = write(x, 64, [(1 << 63) - back], cap, True)
+    want = np.full_like(got, 0xA5)
+    for t in range(min(s, back)):
+        want[0, ((1 << 63) - back + t) % cap] = write_rows(x, 64)[0, t]
+    assert same(got, want)
