@@ -460,7 +460,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
         mbar_init(&sm.p_ready, AK_SOFT);
         mbar_init(&sm.o_done, 1);
         *s_large = 0;
-        *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses
+        *s_abort = (smem_u32(smem) & 1023u) != 0;        // the swizzle goes by addresses: code 57, below
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid < H) sm.m[tid] = AK_NONE;
@@ -519,7 +519,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
 
     // A wait that runs out sets the abort flag, after which every other wait gives up soon; all loops and barriers are gone
     // through all the same, so that no thread is left waiting, and nothing is written.
-    int fail = 0;
+    int fail = tid == 0 && (smem_u32(smem) & 1023u) ? 57 : 0;
     uint32_t done = 0;                                   // tiles of this CTA so far
     bool more = false;
     auto settle = [&]() {                                // cur has been asked for: the first tile from it on with a record

@@ -2,8 +2,10 @@
 import numpy as np
 import pytest
 
+from _gpu import lib, ok
 from _kv8 import write_rows
-from test_gpu_kv8 import rows, same, write
+from test_gpu_kv8 import Case, rows, same, write
+from test_gpu_wait_status import plant
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +18,21 @@ def test_a_ring_at_the_end_of_the_numbers_keeps_the_last_row_that_has_an_entry(b
     for t in range(min(s, back)):
         want[0, ((1 << 63) - back + t) % cap] = write_rows(x, 64)[0, t]
     assert same(got, want)
+
+
+@pytest.mark.parametrize("code", [51, 57])
+def test_a_code_in_the_status_word_stays_until_it_is_read(code):
+    """Planted by the host, as the attention's waits (51 to 56) and its look at its own layout (57) would leave it: a call that only
+    enqueues neither takes nor covers it."""
+    import torch
+    L, c = lib(), Case(3, n=200, seqs=2).put()
+    o = torch.empty(c.rows, c.h, c.d, device="cuda")
+    plant(code)
+    try:
+        ok(c.call(o), "attn")
+        torch.cuda.synchronize()
+        assert L.apus_cuda_kernel_status(0) == code
+    finally:
+        left = L.apus_cuda_kernel_status(1)
+    assert left == code and L.apus_cuda_kernel_status(0) == 0
+    c.check(c.out())
