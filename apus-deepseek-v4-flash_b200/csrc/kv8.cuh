@@ -8,7 +8,8 @@
 //   [d - rd codes][rd BF16][(d - rd) / 64 UE8M0 bytes, zeros up to a multiple of 16]
 //
 // d and rd are multiples of 64, so every part starts on a 64-byte multiple and the scales lie in one 16-byte piece.
-// Scale byte 255 marks a group that held an infinity or a NaN: all of it reads back as NaN.
+// Scale byte 255 marks a group that held an infinity or a NaN: all of it reads back as NaN.  Codes 0x7f and 0xff (E4M3's NaN), which
+// the writer stores under no other scale, are not looked for and count as +-480: integer instructions bound the readers.
 #pragma once
 #include "common.cuh"
 

@@ -517,8 +517,10 @@ int apus_cuda_sparse_attn_batch_dev(const float *q, const float *sink, int h, in
  *   [d - rd E4M3 codes][rd BF16: the rotated channels][one UE8M0 scale per 64 codes, zeros]
  * Codes and scales are those of apus_cuda_fp8_qat_sim (c/attn.h:290-369), so rows that have been
  * through it, as the model's window rows and compressed entries have, are held exactly.  A group
- * of 64 with an infinity or a NaN in it reads back as NaN.  d: a multiple of 64 up to 512; rd: 0
- * or 64, below d (0 bytes and a message otherwise).
+ * of 64 with an infinity or a NaN in it reads back as NaN: its scale byte is 255.  NaN is said by
+ * the scale alone: the code bytes 0x7f and 0xff, which apus_cuda_kv8_write_dev stores under no
+ * other scale, are not looked for and count as 480 and -480 times it, in reading and in attention.
+ * d: a multiple of 64 up to 512; rd: 0 or 64, below d (0 bytes and a message otherwise).
  * A cache is the caller's device memory: n_seq sequences of `cap` records, sequence b from record
  * b * stride on.  All pointers are device pointers; caches, queries and outputs start on 16-byte
  * boundaries, f32 rows that are written or read on 32-byte ones.  Work is enqueued on `stream`;

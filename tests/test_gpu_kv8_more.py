@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 
 from _gpu import lib, ok
-from _kv8 import write_rows
-from test_gpu_kv8 import Case, rows, same, write
+from _kv8 import read_rows, write_rows
+from test_gpu_kv8 import Case, read, rows, same, write
 from test_gpu_wait_status import plant
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +36,20 @@ def test_a_code_in_the_status_word_stays_until_it_is_read(code):
         left = L.apus_cuda_kernel_status(1)
     assert left == code and L.apus_cuda_kernel_status(0) == 0
     c.check(c.out())
+
+
+@pytest.mark.parametrize("scale", [3, 120, 127, 140])
+def test_codes_of_nan_count_as_480_where_the_scale_is_a_number(scale):
+    """In reading, where the scale is one that BF16 products hold or not, and in attention."""
+    c = Case(9, n=100, seqs=2, nb=60, na=0, holes=0.0)
+    c.kv_b[:, :, 5::7] = 0x7f
+    c.kv_b[:, :, 3::64] = 0xff
+    c.kv_b[:, :, 448:576] = 0
+    c.kv_b[:, :, 576:583] = scale
+    val = read_rows(c.kv_b, 512, 64)
+    assert np.abs(val).max() == 480 * 2.0 ** (scale - 127)
+    for bf16 in (False, True):
+        assert same(read(c.kv_b, 512, 64, s=60, bf16=bf16), val)
+    if scale > 16:                                            # else the values are below what an attention has to see
+        c.scale *= 2.0 ** (127 - scale - 9)
+        c.check(c.out())
