@@ -68,15 +68,17 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 }
 
 // ---- the kernel ------------------------------------------------------------------------------------------------------
-// One query row has 64 heads on the same latent rows: 256 operations for every byte of the cache, where this GPU's ratio of
-// tensor rate to memory rate is 253.  So both contractions go to the tensor cores (tcgen05, BF16 operands, f32 sums), a
-// cache row is fetched and dequantised once for all heads, and it serves as key and as value from the same place:
+// One query row has 64 heads on the same latent rows: 225 operations for every byte of a record (4 x 64 x 512 over 583), where
+// this GPU's ratio of tensor rate to memory rate is 253 and that of its FP32 pipes some 10.  So both contractions go to the
+// tensor cores (tcgen05, BF16 operands, f32 sums), a cache row is fetched and dequantised once for all heads of a CTA, and it
+// serves as key and as value from the same place:
 //
 //   S^T[token, head]   = K[token, ch] Q[head, ch]^T     A = 128 rows as they lie (K-major),  B = the queries
 //   O^T[ch, head]     += V[token, ch]^T P[token, head]   A = the same rows (MN-major),         B = the numerators
 //
 // With tokens, then channels as the 128 rows of an instruction, the heads are its columns (64, 32 or 16 in a CTA:
-// attn_kv8_shape) and no instruction runs half empty.  A group of codes times its power of two is a BF16 value exactly (4
+// attn_kv8_shape).  The scores of a short tile (a CTA's share may be 16 tokens) leave rows of theirs unused, the output does not:
+// its rows are channels, and its steps end with the tokens.  A group of codes times its power of two is a BF16 value exactly (4
 // significant bits), so nothing is rounded before the products.  A token is a TMEM lane, so that a thread turns one token's
 // scores into numerators for 32 heads and stores them as one contiguous piece of a row of P.
 //
@@ -105,11 +107,11 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // gathered rows arrive at 3.4 TB/s over the GPU; with 60 KB, at 6.6.  (The 16 rows that an instruction reads behind a panel
 // are the next panel's; what comes of them is masked.)
 //
-// A tile takes 6,000 cycles with 64 heads (5,300 with 32, 5,200 with 16).  In 4,000 of them shared memory is busy: 60 MMAs
-// read 6 KB each at 128 bytes a cycle, and the rows' 112 KB are written while the MMAs of the tile before, panel pair by
-// panel pair, leave their place.  In the other 2,000 the tensor cores wait for the numerators.  (Two tiles of 64 and 48
-// tokens in turn, the one's scores under the other's softmax, took 7,300 where it was 6,300 so: an instruction of 64 rows
-// takes as long as one of 128.)
+// A tile takes 3.2 to 3.5 us with 64 heads (2.8 to 3.1 with 32, 2.8 with 16; lists of 5 to 35 tiles), 6,200 cycles by ncu's
+// count.  In 4,000 of them shared memory is busy: 60 MMAs read 6 KB each at 128 bytes a cycle, and the rows' 112 KB are written
+// while the MMAs of the tile before, panel pair by panel pair, leave their place.  In the other 2,200 the tensor cores wait for the
+// numerators.  (Two tiles of 64 and 48 tokens in turn, the one's scores under the other's softmax, took 7,300 where it was 6,300
+// so: an instruction of 64 rows takes as long as one of 128.)
 constexpr int AK_TILE = 112, AK_HEADS = 64;             // of the largest CTA
 constexpr int AK_SOFT = 8, AK_ROWS = AK_TILE / 16, AK_MMA = AK_SOFT + 2 * AK_ROWS, AK_THREADS = 32 * (AK_MMA + 1);   // warps by role
 constexpr int AK_PANEL = AK_TILE * 128, AK_Q_OFF = 8 * AK_PANEL;
@@ -177,11 +179,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float lg2(float x) {
     float r;
     asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 // Squares of eight BF16 values added to two sums.  Rounding keeps order, so a sum is not below any of its squares: 2^64 or more
@@ -848,17 +845,17 @@ const AkSize ak_sizes[AK_SIZES] = {{64, Ak<64>::SMEM, {attn_kv8_kernel<false, 64
 // 16 CTAs that the GPU holds at once (148, 74, 33, 15 and 7).  Fewer heads per CTA do the work on the candidates' rows once
 // more for every block of heads, but where SMs would have nothing to do every step of a row is shorter; more CTAs per row take
 // fewer tiles each and have a join.  The rule takes the least of: turns in which the GPU takes all clusters, times start, join and
-// tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (over 18 shapes its choice was within 1 % of
-// the fastest in 17, 5 % behind in one):
+// tiles of one.  Measured microseconds, 1 / 2 / 4 / 8 / 16 CTAs, * where the rule goes (when its times were fitted, its choice was
+// within 1 % of the fastest in 17 of 18 shapes, 5 % behind in one; of these eight it is the fastest in seven, 2 % behind in one).
 //                              64 heads per CTA                    32                                  16
-//   1 row of 640 candidates   26.5   21.4   18.9   14.5   14.2    22.8   17.9   15.0   11.7   11.9    21.6   16.8   13.5   10.9*  11.3
-//   6 of 640                  27.6   22.4   19.8   15.4   15.1    23.3   18.1   15.4   12.0*  23.1    21.9   17.0   13.7   21.1   42.1
-//   16 of 640                 28.9   23.8   19.9   29.3   42.9    24.0   19.1   15.6*  33.2   56.0    22.4   17.7   26.1   51.1    104
-//   32 of 640                 29.0   23.9   20.3   43.6   73.2    24.1   19.3*  29.3   55.0    113    22.5   33.5   51.0   91.6
-//   1,024 of 640             199.2*                                332                                 621
-//   1 of 8,320                 238    129   71.4   42.3   28.4     214    115   62.5   36.8   24.2     208    111   60.1   35.6   23.1*
-//   32 of 8,320                246    136   77.1*   128    143     225    121    135    188    242     214    227    251    321
-//   5 of 128, 8 heads         12.6   12.6   12.7   12.3   12.5    10.8   11.1   10.7   11.0   11.2    10.0*  10.7   10.1   10.5   10.8
+//   1 row of 640 candidates   27.1   21.4   18.7   14.2   14.0    23.2   17.8   15.0   11.6   11.9    22.1   16.8   13.5   10.8*  11.1
+//   6 of 640                  28.4   22.4   19.7   15.2   15.0    23.6   18.1   15.2   12.0*  23.1    22.4   17.2   13.7   21.0   42.1
+//   16 of 640                 29.9   24.1   19.8   29.4   42.9    24.4   19.1   15.4*  33.3   56.3    22.9   17.7   26.2   51.0    104
+//   32 of 640                 29.9   24.2   20.0   43.7   73.4    24.5   19.3*  29.1   55.4    113    23.1   33.7   51.3   91.5
+//   1,024 of 640             204.1*                                336                                 631
+//   1 of 8,320                 249    134   73.7   43.3   28.9     217    117   63.6   37.3   24.6     212    114   61.1   36.2   23.4*
+//   32 of 8,320                252    138   78.8*   130    145     222    120    134    187    243     212    224    248    319
+//   5 of 128, 8 heads         12.8   12.7   12.7   12.5   12.7    10.8   11.1   10.6   10.9   11.1    10.2*  10.5   10.0   10.4   10.6
 int attn_kv8_shape(int idxw, int h, int rows, const int (&slots)[AK_SIZES][5], int *cluster, int *unit, int *ahead) {
     double best = 0;
     int which = 0;

@@ -19,11 +19,6 @@ namespace {
 
 constexpr int KV8_WARPS = 8, KV8_STEP = 256, KV8_STEPS = KV8_MAX_D / KV8_STEP;
 
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 // 8 values of f32 in one access (32-byte boundaries)
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
     asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -36,7 +31,8 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 
 // Row t of sequence b goes to entry pos[b] + t of that sequence's cache, modulo `cap` in a ring.  Of the rows of one call
 // that share a place in a ring only the last is written, so that the result is that of writing them one by one.
-// B200, 65,536 rows of 512: BF16 19.6 us, f32 25.8 us (5.4 and 6.7 TB/s).
+// B200, 65,536 rows of 512, eight sets of buffers in turn so that L2 holds none: BF16 19.6 us, f32 25.7 us (5.4 and 6.7 TB/s, where a
+// plain copy moves 6.55: three quarters of the f32 traffic are reads).
 template <bool BF16>
 __global__ void __launch_bounds__(32 * KV8_WARPS)
 kv8_write_kernel(const void *x, int d, int rd, uint32_t rows, uint32_t s, const int64_t *pos, const int32_t *counts, bool ring,
@@ -104,7 +100,7 @@ kv8_write_kernel(const void *x, int d, int rd, uint32_t rows, uint32_t s, const 
     if (lane == 0) *reinterpret_cast<uint4 *>(rec + kv8_scale_off(d, rd)) = make_uint4(sc[0], sc[1], 0u, 0u);
 }
 
-// B200, 65,536 rows of 512: to BF16 18.5 us, to f32 27.5 us (5.7 and 6.3 TB/s).
+// B200, 65,536 rows of 512, measured likewise: to BF16 18.6 us, to f32 27.7 us (5.7 and 6.2 TB/s).
 __global__ void __launch_bounds__(32 * KV8_WARPS)
 kv8_read_kernel(const uint8_t *cache, int d, int rd, long long cap, long long stride, uint32_t rows, uint32_t s, const int32_t *idx,
                 long long first, void *out, bool bf16) {

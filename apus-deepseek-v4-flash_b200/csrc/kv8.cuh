@@ -33,6 +33,11 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // Four codes -> four BF16 values in the order 0 2 | 1 3, times 2^-120 and the factor in `f` (a BF16 value twice).  Exponent
 // and significand move to their places in BF16 (whose bias is 120 larger; a subnormal code becomes a subnormal value) and
 // the sign goes into the factor.  The order saves the byte permutations: integer instructions issue every other cycle, and
