@@ -108,3 +108,15 @@ def test_reading_by_index_into_bf16_rows(d, rd):
     idx = rng.integers(-2, 55, (3, 77))
     want = np.where(((idx >= 0) & (idx < 50))[..., None], read_rows(rec, d, rd)[np.arange(3)[:, None], np.clip(idx, 0, 49)], 0)
     assert same(read(rec, d, rd, idx=idx, bf16=True), want) and same(read(rec, d, rd, idx=idx), want)
+
+
+@pytest.mark.parametrize("per,entries", [(200, 0), (6, 0), (200, 1000), (90, 7)])
+def test_chunks_of_window_layers_and_of_heavily_compressed_ones(per, entries):
+    """Two prompts; row t attends rows t .. t + 127 of its window buffer and the entries that were complete at its position."""
+    seqs, win = 2, 128
+    c = Case(per + entries, n=win + entries, seqs=seqs, per=per, na=win - 1 + per, nb=entries, holes=0.0)
+    t = np.tile(np.arange(per), seqs)[:, None]
+    have = entries - 4 + t * 4 // per                         # some complete within the chunk
+    e = np.arange(entries)
+    c.idx[:] = np.concatenate((t + np.arange(win), np.where(e < have, c.na + e, -1)), 1)
+    c.check(c.out(), sorted({0, 1, per - 1, per, c.rows // 2 + 1, c.rows - 1}))
