@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // the first tile's maximum and stays until a score exceeds it by more than AK_SLACK of them, which in f32 and BF16, floating
 // as both are, costs no precision: numerators of 2^-48 to 2^64 are as good as those around 1, and what is below 2^-126 is
 // less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles, by a factor of
-// down to 2^-190 and beyond, which f32 does not hold: numerators of 2^64 before are 2^-14 of the new largest one at a factor of
+// any size, 2^-112 at most, which f32 may not hold: numerators of 2^64 before are 2^-14 of the new largest one at a factor of
 // 2^-126, so it is applied as two.  (With the reference at the maximum itself, heads whose scores spread over some 50 powers
 // of two set it anew in three of nineteen tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)
 // Where a row has values of 2^32 or more, numerators of 2^64 would take the sums out of f32: from there on references are set
@@ -246,7 +246,7 @@ __device__ __forceinline__ uint64_t ak_desc_mn(uint32_t saddr, int width) {
            (uint64_t)(width == 128 ? 2 : width == 64 ? 4 : 6) << 61;
 }
 
-// exp(scale s - reference).  The product is rounded as it was when the reference was set from it: left exact, in one instruction,
+// 2^(scale s - reference).  The product is rounded as it was when the reference was set from it: left exact, in one instruction,
 // it is some powers of two above or below from 2^27 on, and more than f32 holds from 2^31 on.  (1,024 rows of 640 candidates: one
 // instruction 203.4 us, two 204.1.)
 __device__ __forceinline__ float ak_numerator(uint32_t s, float cs, float reference) {
@@ -595,7 +595,7 @@ attn_kv8_kernel(const AttnKv8Args a) {
             const int held = (min(a.unit, a.idxw - tile * a.unit) + 15) & ~15;   // rows that the MMAs read
             tile += C;
             cur.load(a, ids, tile, lane);
-            rows.convert(0, n_codes, s_large);                    // before there is room for it, while the tile before is worked on
+            rows.convert(0, n_codes, s_large);           // before there is room for it, while the tile before is worked on
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (2 * i >= n) break;
