@@ -85,9 +85,9 @@ __device__ __forceinline__ uint32_t ldg4_if(const uint8_t *p, bool yes) {
 // The softmax is one pass with a reference per head instead of the running maximum: it is set AK_ABOVE powers of two above
 // the first tile's maximum and stays until a score exceeds it by more than AK_SLACK of them, which in f32 and BF16, floating
 // as both are, costs no precision: numerators of 2^-48 to 2^64 are as good as those around 1, and what is below 2^-126 is
-// less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles, by a factor of
-// any size, 2^-112 at most, which f32 may not hold: numerators of 2^64 before are 2^-14 of the new largest one at a factor of
-// 2^-126, so it is applied as two.  (With the reference at the maximum itself, heads whose scores spread over some 50 powers
+// less than 2^-77 of the largest one.  Only then is the accumulator scaled, which takes 3,000 to 4,000 cycles, by a factor
+// that f32 may not hold: at 2^-126, numerators of 2^64 before still are 2^-14 of the new largest one.  So it is applied as
+// two.  (With the reference at the maximum itself, heads whose scores spread over some 50 powers
 // of two set it anew in three of nineteen tiles: 1,024 rows of 640 candidates 223 us, 208 so; one row of 8,320 33.1 and 30.1.)
 // Where a row has values of 2^32 or more, numerators of 2^64 would take the sums out of f32: from there on references are set
 // so that no numerator is above 1, as in a softmax with the maximum at hand.  Sums of numerators stay in each thread until the
